@@ -237,6 +237,72 @@ int opal_ingest_scan(opal_ctx *ctx, const uint8_t *d_text, uint64_t nbytes, uint
 int opal_eval_counts(opal_ctx *ctx, const int32_t *d_pred, const int32_t *d_ref, uint64_t n, uint32_t n_classes,
                      uint64_t *d_correct, uint64_t *d_total);
 
+/* ---- score head: operators behind the per-class scores ------------------------------------------------------
+ * NO COUNTERPART IN THE REFERENCE, whose answer is the argmax of K independent regressors (opal.py:449-469).  They put a trained
+ * head on the scores opal_predict writes: z = layer norm of the scores, logits = z + W2 act(W1 z + b1) + b2, softmax cross
+ * entropy; `opal train --head` and `opal predict` use them, and each can be called by itself.
+ *
+ * A matrix is a device pointer, an element type and a row stride `ld` in ELEMENTS (ld >= its columns, at most 2^21; any element
+ * alignment; rows of 16-byte alignment are faster for 16- and 32-bit products).  Columns, `in`, `out` and K: 1 .. 2^20; n < 2^31
+ * rows, n = 0 is allowed (sums over no rows are zeros).  What lies between two rows is neither used nor written.
+ * Parameters, statistics, losses and weight gradients are float32; sums are taken in float32 and a result is rounded once, to
+ * its own type.  An output may be one of the inputs only where that is said.  The calls allocate nothing, do not synchronise and can be
+ * captured into a HIP graph; workspaces are the caller's (16-byte aligned; calls that may overlap need one each), and results are
+ * the same bits every time.                                                                                        */
+#define OPAL_F32 0
+#define OPAL_F16 1
+#define OPAL_BF16 2
+#define OPAL_ACT_NONE 0
+#define OPAL_ACT_RELU 1
+#define OPAL_ACT_SILU 2     /* v / (1 + exp(-v))                                                       */
+#define OPAL_ACT_GELU 3     /* v / (1 + exp(-2 sqrt(2/pi) (v + 0.044715 v^3))): the tanh form          */
+
+/* y = (x - mean) rstd gamma + beta per row; mean = sum(x)/cols, rstd = 1/sqrt(sum((x - mean)^2)/cols + eps), eps > 0.
+ * d_gamma / d_beta [cols]: NULL = 1 / 0.  d_mean / d_rstd [n]: NULL = not wanted (opal_layer_norm_backward needs them).
+ * y may be x (same type and ld).                                                                                   */
+int opal_layer_norm(opal_ctx *ctx, const void *d_x, int x_type, uint64_t ldx, const float *d_gamma, const float *d_beta,
+                    uint64_t n, uint32_t cols, float eps, void *d_y, int y_type, uint64_t ldy, float *d_mean, float *d_rstd);
+
+/* With h = dy gamma and xh = (x - mean) rstd:  dx = rstd (h - mean(h) - xh mean(h xh)),  dgamma = sum over rows of dy xh,
+ * dbeta = sum over rows of dy.  d_dx, d_dgamma, d_dbeta: NULL = not wanted; dx may be dy or x (same type and ld).  d_work:
+ * opal_layer_norm_backward_workspace(n, cols) bytes, needed for dgamma / dbeta (OPAL_ERANGE when smaller).           */
+uint64_t opal_layer_norm_backward_workspace(uint64_t n, uint32_t cols);
+int opal_layer_norm_backward(opal_ctx *ctx, const void *d_dy, int dy_type, uint64_t lddy, const void *d_x, int x_type, uint64_t ldx,
+                             const float *d_gamma, const float *d_mean, const float *d_rstd, uint64_t n, uint32_t cols, void *d_dx,
+                             int dx_type, uint64_t lddx, float *d_dgamma, float *d_dbeta, void *d_work, uint64_t work_bytes);
+
+/* y[n, out] = act(x[n, in] w[out, in]^T + bias) + res.  x and w share one type, in which the value before the activation is
+ * stored too (d_pre [n, out], what opal_linear_grad_input takes).  d_bias [out], d_res [n, out], d_pre: NULL = without.
+ * y may be res (same type and ld).                                                                                  */
+int opal_linear(opal_ctx *ctx, const void *d_x, uint64_t ldx, const void *d_w, uint64_t ldw, int type, const float *d_bias,
+                int activation, const void *d_res, int res_type, uint64_t ldr, uint64_t n, uint32_t in, uint32_t out,
+                void *d_y, int y_type, uint64_t ldy, void *d_pre, uint64_t ldp);
+
+/* dx[n, in] = (dy[n, out] w[out, in]) act'(pre[n, in]) + res[n, in]: the gradient of a product's input, through the activation that
+ * made that input (pre: its value before the activation, in the type of dy and w) and with the share of a skip connection added.
+ * activation = OPAL_ACT_NONE: pre is not read.  dx may be res (same type and ld).                                     */
+int opal_linear_grad_input(opal_ctx *ctx, const void *d_dy, uint64_t lddy, const void *d_w, uint64_t ldw, int type, const void *d_pre,
+                           uint64_t ldp, int activation, const void *d_res, int res_type, uint64_t ldr, uint64_t n, uint32_t in,
+                           uint32_t out, void *d_dx, int dx_type, uint64_t lddx);
+
+/* dw[out, in] = dy[n, out]^T x[n, in] and dbias[out] = sum over rows of dy, in float32; either may be NULL.  dy is the gradient
+ * before the activation.  d_work: opal_linear_grad_weight_workspace(n, in, out, type) bytes (OPAL_ERANGE when smaller).  */
+uint64_t opal_linear_grad_weight_workspace(uint64_t n, uint32_t in, uint32_t out, int type);
+int opal_linear_grad_weight(opal_ctx *ctx, const void *d_dy, uint64_t lddy, const void *d_x, uint64_t ldx, int type, uint64_t n, uint32_t in,
+                            uint32_t out, float *d_dw, uint64_t lddw, float *d_dbias, void *d_work, uint64_t work_bytes);
+
+/* Cross entropy of softmax(scores) against class ids 1..K (as in opal_train_batch); label 0 = a row without a known class, whose
+ * loss and gradient are 0.  Any other label counts as 0, and the next opal_sync returns OPAL_EINVAL with the number of them.
+ * d_loss[i] = log sum exp(s_i) - s_i[label];  grad = scale (softmax(s_i) - [class is the label]).  Either may be NULL.
+ * Scores of -inf are classes that are ruled out (probability 0); in a row of nothing else the gradient is 0 and the loss +inf.
+ * NaN or +inf among a labelled row's scores makes its loss and gradient NaN.  grad may be scores (same type and ld).    */
+int opal_softmax_loss(opal_ctx *ctx, const void *d_scores, int type, uint64_t ld, uint64_t n, uint32_t K, const int32_t *d_labels,
+                      float scale, float *d_loss, void *d_grad, int grad_type, uint64_t ldg);
+
+/* The answer: d_out_class[i] = 1-based class of the highest score (ties: the lowest class; NaN never wins; class 1 when nothing is
+ * above -inf), d_out_prob[i] (may be NULL) = its softmax probability (0 when nothing is above -inf).                   */
+int opal_softmax_class(opal_ctx *ctx, const void *d_scores, int type, uint64_t ld, uint64_t n, uint32_t K, int32_t *d_out_class, float *d_out_prob);
+
 /* Name of the scoring-kernel variant opal_predict would launch for the current K (for profiles/bench).   */
 const char *opal_predict_kernel_name(opal_ctx *ctx);
 

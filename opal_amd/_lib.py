@@ -14,6 +14,7 @@ OPAL_EHIP = -5
 OPAL_ERANGE = -34
 RAW_FLAG = 0x80000000
 VW_CONSTANT = 11650396
+OPAL_F32, OPAL_F16, OPAL_BF16 = 0, 1, 2
 
 # every symbol include/opal_hip.h declares: (restype, argtypes)
 _vp, _u64, _u32, _i32, _int, _f32, _f64 = C.c_void_p, C.c_uint64, C.c_uint32, C.c_int32, C.c_int, C.c_float, C.c_double
@@ -54,6 +55,15 @@ PROTOTYPES = {
     "opal_load_weights_sparse": (_int, [_vp, _vp, _vp, _u64, _int, _int]),
     "opal_get_accumulators": (_int, [_vp, _vp, _int]),
     "opal_load_accumulators_sparse": (_int, [_vp, _vp, _vp, _u64]),
+    "opal_layer_norm": (_int, [_vp, _vp, _int, _u64, _vp, _vp, _u64, _u32, _f32, _vp, _int, _u64, _vp, _vp]),
+    "opal_layer_norm_backward_workspace": (_u64, [_u64, _u32]),
+    "opal_layer_norm_backward": (_int, [_vp, _vp, _int, _u64, _vp, _int, _u64, _vp, _vp, _vp, _u64, _u32, _vp, _int, _u64, _vp, _vp, _vp, _u64]),
+    "opal_linear": (_int, [_vp, _vp, _u64, _vp, _u64, _int, _vp, _int, _vp, _int, _u64, _u64, _u32, _u32, _vp, _int, _u64, _vp, _u64]),
+    "opal_linear_grad_input": (_int, [_vp, _vp, _u64, _vp, _u64, _int, _vp, _u64, _int, _vp, _int, _u64, _u64, _u32, _u32, _vp, _int, _u64]),
+    "opal_linear_grad_weight_workspace": (_u64, [_u64, _u32, _u32, _int]),
+    "opal_linear_grad_weight": (_int, [_vp, _vp, _u64, _vp, _u64, _int, _u64, _u32, _u32, _vp, _u64, _vp, _vp, _u64]),
+    "opal_softmax_loss": (_int, [_vp, _vp, _int, _u64, _u64, _u32, _vp, _f32, _vp, _vp, _int, _u64]),
+    "opal_softmax_class": (_int, [_vp, _vp, _int, _u64, _u64, _u32, _vp, _vp]),
 }
 
 _lib = None

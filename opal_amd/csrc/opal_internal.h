@@ -48,6 +48,9 @@ struct opal_ctx {
     std::string err;
 };
 
+// word of ctx->d_queue (opal_device.h describes the others): labels of opal_softmax_loss calls that name no class, since the last opal_sync
+constexpr int Q_BAD_LABEL = 288;
+
 namespace opal {
 int fail(opal_ctx *ctx, int code, const std::string &msg);
 // the deterministic trainer (opal_dtrain.hip)

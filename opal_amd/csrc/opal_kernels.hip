@@ -1245,15 +1245,22 @@ extern "C" int opal_sync(opal_ctx *ctx)
     if (!ctx) return opal::fail(nullptr, OPAL_EINVAL, "opal_sync: null ctx");
     // fragments of opal_features / opal_feature_names calls that reached outside their d_reads (queue word Q_BAD): read and
     // cleared on the ctx's own stream, so that a ctx on a stream of its own never serialises against the null stream
-    unsigned long long bad = 0;
+    static_assert(Q_BAD < Q_BAD_LABEL && Q_BAD_LABEL < Q_WORDS, "words of d_queue");
+    constexpr int SPAN = Q_BAD_LABEL - Q_BAD + 1;
+    unsigned long long seen[SPAN] = {};
     OPAL_HIP_CHECK(ctx, hipSetDevice(ctx->device));
-    OPAL_HIP_CHECK(ctx, hipMemcpyAsync(&bad, ctx->d_queue + Q_BAD, sizeof(bad), hipMemcpyDeviceToHost, ctx->stream));
+    OPAL_HIP_CHECK(ctx, hipMemcpyAsync(seen, ctx->d_queue + Q_BAD, sizeof(seen), hipMemcpyDeviceToHost, ctx->stream));
     OPAL_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
-    if (bad) {
-        OPAL_HIP_CHECK(ctx, hipMemsetAsync(ctx->d_queue + Q_BAD, 0, sizeof(bad), ctx->stream));
+    const unsigned long long bad = seen[0], labels = seen[Q_BAD_LABEL - Q_BAD];
+    if (bad || labels) {
+        OPAL_HIP_CHECK(ctx, hipMemsetAsync(ctx->d_queue + Q_BAD, 0, sizeof(seen), ctx->stream));
         OPAL_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
-        return opal::fail(ctx, OPAL_EINVAL, std::to_string(bad) + " fragment(s) of the emit calls since the last opal_sync reach outside d_reads "
-                                            "(offset + length beyond reads_bytes): their features were written as 0xffffffff / NUL names");
+        std::string msg;
+        if (bad) msg = std::to_string(bad) + " fragment(s) of the emit calls since the last opal_sync reach outside d_reads "
+                                             "(offset + length beyond reads_bytes): their features were written as 0xffffffff / NUL names";
+        if (labels) msg += std::string(bad ? "; " : "") + std::to_string(labels) + " label(s) of the opal_softmax_loss calls since the last opal_sync are "
+                                                          "neither 0 nor a class 1..K: those rows count as unlabelled";
+        return opal::fail(ctx, OPAL_EINVAL, msg);
     }
     return OPAL_OK;
 }

@@ -1,0 +1,389 @@
+// Matrix products of the score head: the tile kernel behind opal_linear, opal_linear_grad_input and opal_linear_grad_weight, and
+// what its three translation units (one per element type) share.
+//
+//   C[m, n] = sum_k A(m, k) B(n, k), sums in 32 bits, then the epilogue of the product in question:
+//     FWD  y  = act(x W^T + b) + r      A = x  [M, K], B = W [N, K]: the k of a row lie side by side in both ("KC")
+//     GIN  dx = (dy W) act'(pre) + r    A = dy [M, K], B = W [K, N]: the n of a k lie side by side in W ("MC")
+//     GWT  dW = dy^T x                  A = dy [K, M], B = x [K, N]: both MC, and K is the number of rows of the batch
+//
+// A block owns a BM x BN tile of C and walks k in steps of 128 bytes (64 elements of 16 bits, 32 of 32).  Both operands' tiles
+// go to LDS as 16-byte chunks, twice buffered, and from there to registers as operands of v_mfma_f32_32x32x16 (16 bits) or
+// v_mfma_f32_32x32x2_f32.  The MFMA's first operand is B and its second A, so a lane ends up with four neighbouring n of one m.
+#pragma once
+#include "opal_head.h"
+
+namespace opal_head {
+
+enum Product { FWD = 0, GIN = 1, GWT = 2 };
+enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
+
+struct Linear {
+    const char *a, *b;
+    uint64_t lda, ldb;            // row strides in elements
+    uint64_t M, N, K;
+    uint64_t ksplit;              // k handled by one block (a multiple of the step; >= K without a split)
+    uint32_t tm, tn, splits;      // tiles along M and N, splits of K
+    const float *bias;            // [N] or null
+    const void *res; int res_type; uint64_t ldr;
+    void *y; int y_type; uint64_t ldy;
+    uint64_t y_split;             // elements between two splits' outputs
+    const void *pre_in; void *pre_out; uint64_t ldp;   // the element type of the product
+    int act;
+};
+
+constexpr float GELU_A = 1.5957691216057308f, GELU_B = 0.044715f;   // 2 sqrt(2 / pi), and the cubic term of the tanh form
+
+// v_exp_f32 and v_rcp_f32 are good to 1 ulp; the argument's rounding costs |z| 2^-24 of the result
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896f * z)); }
+
+__device__ __forceinline__ float act_value(float v, int act)
+{
+    if (act == ACT_RELU) return v > 0.f || v != v ? v : 0.f;
+    if (act == ACT_SILU) return v * sigmoid(v);
+    if (act == ACT_GELU) return v * sigmoid(GELU_A * (v + GELU_B * v * v * v));
+    return v;
+}
+
+__device__ __forceinline__ float act_slope(float v, int act)
+{
+    if (act == ACT_RELU) return v > 0.f ? 1.f : 0.f;
+    const float c = fminf(fmaxf(v, -64.f), 64.f);      // beyond it p is 0 or 1 and c^2 p (1 - p) must not become 0 inf
+    if (act == ACT_SILU) {
+        const float p = sigmoid(v);
+        return p + c * p * (1.f - p);
+    }
+    const float p = sigmoid(GELU_A * (v + GELU_B * v * v * v));
+    return p + c * p * (1.f - p) * GELU_A * (1.f + 3.f * GELU_B * c * c);
+}
+
+#ifdef __HIP_DEVICE_COMPILE__
+#define OPAL_LDS __attribute__((address_space(3)))
+#endif
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int STEP_BYTES = 128;          // of k per row and step
+
+// Where chunk c of row r of a KC tile lies within the row's eight: rows r and r + 1 share 256 bytes (all banks), the rotation by
+// r >> 1 then spreads the same c of 16 rows over all 16 places, which is what a fragment read asks for.
+__device__ __forceinline__ int swizzle_kc(int r) { return (r >> 1) & 7; }
+// The same for the k-th line of an MC tile of R columns (in chunks).  16 bits: a transposing read takes 64 bytes of lines
+// k .. k+3 and k+8 .. k+11; four lines get the four quarters of the banks (lines of 128 bytes: the two halves).
+// 32 bits: a read takes 128 bytes of lines k and k + 4.
+template <int ES, int R> __device__ __forceinline__ int swizzle_mc(int k)
+{
+    if constexpr (ES == 4) return ((k >> 2) & 1) << 3;
+    else if constexpr (R * ES >= 256) return (k & 3) << 2;
+    else return ((k >> 1) & 1) << 2;
+}
+
+// One operand's tile: R rows (m or n) of one step of k.
+template <class T, int R, bool KC, int NT, bool DMA> struct Operand {
+    static constexpr int ES = sizeof(T), EPC = 16 / ES, STEP = STEP_BYTES / ES;
+    static constexpr int CHUNKS = R * 8, PER = CHUNKS / NT, LINE = KC ? 8 : R / EPC;   // LINE: chunks of a line
+    static_assert(CHUNKS % NT == 0, "whole chunks per thread");
+    const char *base;             // element (row r0, k0) of the matrix
+    uint64_t ld;                  // bytes
+    int rows;                     // of the tile, within the matrix
+    u32x4 reg[DMA ? 1 : PER];
+
+    __device__ __forceinline__ static int swz(int line) { return KC ? swizzle_kc(line) : swizzle_mc<ES, R>(line); }
+
+    // Starts the loads of the step that begins at `base`, of which krem values of k are left.
+    __device__ __forceinline__ void fetch(char *lds, uint64_t krem)
+    {
+        const int tid = threadIdx.x;
+        const int kval = (int)(krem < (uint64_t)STEP ? krem : (uint64_t)STEP);
+        if constexpr (DMA) {
+#ifdef __HIP_DEVICE_COMPILE__
+            // 16-byte aligned matrix and lines: whole chunks straight into LDS.  The buffer ends with the chunk that holds the
+            // step's last element; lines behind it read as zeros.  A chunk that begins within the matrix lies whole in its
+            // page; what it holds behind the matrix's edge is either never used (columns) or cleared by clear_tail (k).
+            const uint32_t len = (uint32_t)((((uint64_t)(KC ? rows : kval) - 1) * ld + (uint64_t)(KC ? kval : rows) * ES + 15) & ~15ull);
+            auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, (short)0, (int)len, 0x00020000);
+            const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int q = i * NT + tid, line = q / LINE, c = (q % LINE) ^ swz(line);
+                uint32_t off = (uint32_t)line * (uint32_t)ld + (uint32_t)c * 16u;
+                if (KC && c * EPC >= kval) off = 0x80000000u;      // behind every buffer (len < 2^31)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (OPAL_LDS void *)(lds + (i * NT + wave * WAVE) * 16), 16, (int)off, 0, 0, 0);
+            }
+#endif
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int q = i * NT + tid, line = q / LINE, c = (q % LINE) ^ swz(line);
+                const int lines = KC ? rows : kval, width = KC ? kval : rows;
+                const int left = width - c * EPC;
+                const char *p = base + (uint64_t)line * ld + c * 16;
+                u32x4 v = {0, 0, 0, 0};
+                if (line < lines && left > 0) {
+                    if (left >= EPC) {
+                        struct __attribute__((packed, aligned(sizeof(T)))) Any { uint32_t w[4]; };
+                        const Any a = *reinterpret_cast<const Any *>(p);
+                        v = u32x4{a.w[0], a.w[1], a.w[2], a.w[3]};
+                    } else {
+                        if constexpr (ES == 4) {
+#pragma unroll
+                            for (int e = 0; e < EPC - 1; e++)
+                                if (e < left) v[e] = ((const uint32_t *)p)[e];
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < EPC - 1; e++)
+                                if (e < left) v[e / 2] |= (uint32_t)((const uint16_t *)p)[e] << (16 * (e & 1));
+                        }
+                    }
+                }
+                reg[i] = v;
+            }
+        }
+    }
+    __device__ __forceinline__ void commit(char *lds)
+    {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) *reinterpret_cast<u32x4 *>(lds + (i * NT + threadIdx.x) * 16) = reg[i];
+        }
+    }
+    __device__ __forceinline__ void advance() { base += KC ? (uint64_t)STEP_BYTES : (uint64_t)STEP * ld; }
+
+    // The k behind the matrix's edge in the last chunk of each row (KC): whatever lies there must not meet a NaN-free sum.
+    __device__ __forceinline__ static void clear_tail(char *lds, int kval)
+    {
+        if constexpr (KC && DMA) {
+            const int keep = kval % EPC, c = kval / EPC;      // the chunk holds `keep` values of k; the caller checked keep != 0
+            for (int r = threadIdx.x; r < R; r += NT) {
+                T *p = reinterpret_cast<T *>(lds + r * STEP_BYTES + ((c ^ swizzle_kc(r)) * 16));
+#pragma unroll
+                for (int e = 1; e < EPC; e++)
+                    if (e >= keep) p[e] = (T)0.f;
+            }
+        }
+    }
+
+    // Fragment of 32 rows from r0 on, 16-bit types: k = 16 kk + 8 (lane / 32) + 0..7 of row r0 + lane % 32.
+    __device__ __forceinline__ static s16x8 frag16(const char *lds, int r0, int kk)
+    {
+        const int lane = threadIdx.x & 63;
+        if constexpr (KC) {
+            const int r = r0 + (lane & 31), c = kk * 2 + (lane >> 5);
+            return *reinterpret_cast<const s16x8 *>(lds + r * STEP_BYTES + ((c ^ swizzle_kc(r)) * 16));
+        } else {
+            s16x8 v = {};
+#ifdef __HIP_DEVICE_COMPILE__
+            // 16 lanes read four lines of 16 columns, 8 bytes each, and get the four k of one column
+            const int col = r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k = kk * 16 + (lane >> 5) * 8 + h * 4 + ((lane >> 2) & 3);
+                const char *p = lds + k * (R * ES) + (((col >> 3) ^ swizzle_mc<ES, R>(k)) * 16) + (col & 7) * 2;
+                const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((OPAL_LDS s16x4 *)p);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[h * 4 + e] = t[e];
+            }
+#endif
+            return v;
+        }
+    }
+    // 32-bit type: k = 8 j + 4 (lane / 32) + 0..3 of row r0 + lane % 32.
+    __device__ __forceinline__ static f32x4 frag32(const char *lds, int r0, int j)
+    {
+        const int lane = threadIdx.x & 63, r = r0 + (lane & 31);
+        if constexpr (KC) {
+            const int c = j * 2 + (lane >> 5);
+            return *reinterpret_cast<const f32x4 *>(lds + r * STEP_BYTES + ((c ^ swizzle_kc(r)) * 16));
+        } else {
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int k = j * 8 + (lane >> 5) * 4 + e;
+                v[e] = *reinterpret_cast<const float *>(lds + k * (R * ES) + (((r >> 2) ^ swizzle_mc<ES, R>(k)) * 16) + (r & 3) * 4);
+            }
+            return v;
+        }
+    }
+};
+
+template <class T> __device__ __forceinline__ f32x16 mfma16(s16x8 a, s16x8 b, f32x16 c)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    if constexpr (__is_same(T, bf16_t)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+#else
+    return c;
+#endif
+}
+
+// Tile of a block.  Consecutive blocks go to the eight XCDs in turn, each with an L2 of its own; the tiles of an XCD are
+// consecutive ones, the tiles along N of the same rows side by side, so that A's rows are read from HBM once per XCD.
+__device__ __forceinline__ uint32_t xcd_tile(uint32_t b, uint32_t total)
+{
+    const uint32_t x = b & 7u, per = total >> 3, extra = total & 7u;
+    return x * per + (x < extra ? x : extra) + (b >> 3);
+}
+
+template <class T, int P, int BM, int BN, int WM, int WN, bool DMA>
+__global__ __launch_bounds__(WM * WN * WAVE) void linear_kernel(const Linear g)
+{
+    constexpr int NT = WM * WN * WAVE, ES = sizeof(T), STEP = STEP_BYTES / ES;
+    constexpr int FM = BM / WM, FN = BN / WN, TM = FM / 32, TN = FN / 32;     // a wave's part and its fragments
+    using OA = Operand<T, BM, P != GWT, NT, DMA>;
+    using OB = Operand<T, BN, P == FWD, NT, DMA>;
+    constexpr int STAGE = (BM + BN) * STEP_BYTES, EP_LD = FN + 4, EPI = WM * WN * 32 * EP_LD * 4;
+    __shared__ __attribute__((aligned(128))) char lds[2 * STAGE > EPI ? 2 * STAGE : EPI];
+
+    uint32_t t = xcd_tile(blockIdx.x, gridDim.x);
+    const uint32_t tiles = g.tm * g.tn, split = t / tiles;
+    t -= split * tiles;
+    const uint64_t m0 = (uint64_t)(t / g.tn) * BM, n0 = (uint64_t)(t % g.tn) * BN;
+    const uint64_t kbeg = split * g.ksplit, kend = kbeg + g.ksplit < g.K ? kbeg + g.ksplit : g.K;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wm = (wave / WN) * FM, wn = (wave % WN) * FN;
+
+    OA A;
+    OB B;
+    A.ld = g.lda * ES;
+    B.ld = g.ldb * ES;
+    A.rows = (int)(g.M - m0 < (uint64_t)BM ? g.M - m0 : (uint64_t)BM);
+    B.rows = (int)(g.N - n0 < (uint64_t)BN ? g.N - n0 : (uint64_t)BN);
+    A.base = g.a + (P != GWT ? m0 * A.ld + kbeg * ES : kbeg * A.ld + m0 * ES);
+    B.base = g.b + (P == FWD ? n0 * B.ld + kbeg * ES : kbeg * B.ld + n0 * ES);
+
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+
+    uint64_t krem = kend - kbeg;
+    char *cur = lds, *nxt = lds + STAGE;
+    if (krem) {
+        A.fetch(cur, krem);
+        B.fetch(cur + BM * STEP_BYTES, krem);
+        A.commit(cur);
+        B.commit(cur + BM * STEP_BYTES);
+    }
+    while (krem) {
+        __syncthreads();          // the step's chunks are in LDS, and nobody reads the other half any more
+        const bool more = krem > (uint64_t)STEP;
+        if (more) {
+            A.advance();
+            B.advance();
+            A.fetch(nxt, krem - STEP);
+            B.fetch(nxt + BM * STEP_BYTES, krem - STEP);
+        } else if (DMA && P != GWT && krem % OA::EPC) {
+            OA::clear_tail(cur, (int)krem);
+            OB::clear_tail(cur + BM * STEP_BYTES, (int)krem);
+            __syncthreads();
+        }
+        const char *la = cur, *lb = cur + BM * STEP_BYTES;
+        if constexpr (ES == 2) {
+#pragma unroll
+            for (int kk = 0; kk < STEP / 16; kk++) {
+                s16x8 fa[TM], fb[TN];
+#pragma unroll
+                for (int i = 0; i < TM; i++) fa[i] = OA::frag16(la, wm + i * 32, kk);
+#pragma unroll
+                for (int j = 0; j < TN; j++) fb[j] = OB::frag16(lb, wn + j * 32, kk);
+#pragma unroll
+                for (int i = 0; i < TM; i++)
+#pragma unroll
+                    for (int j = 0; j < TN; j++) acc[i][j] = mfma16<T>(fb[j], fa[i], acc[i][j]);
+            }
+        } else {
+#pragma unroll
+            for (int kk = 0; kk < STEP / 8; kk++) {
+                f32x4 fa[TM], fb[TN];
+#pragma unroll
+                for (int i = 0; i < TM; i++) fa[i] = OA::frag32(la, wm + i * 32, kk);
+#pragma unroll
+                for (int j = 0; j < TN; j++) fb[j] = OB::frag32(lb, wn + j * 32, kk);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int i = 0; i < TM; i++)
+#pragma unroll
+                        for (int j = 0; j < TN; j++) {
+#ifdef __HIP_DEVICE_COMPILE__
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j][e], fa[i][e], acc[i][j], 0, 0, 0);
+#endif
+                        }
+            }
+        }
+        if (more) {
+            A.commit(nxt);
+            B.commit(nxt + BM * STEP_BYTES);
+        }
+        char *const s = cur;
+        cur = nxt;
+        nxt = s;
+        krem = more ? krem - STEP : 0;
+    }
+
+    // Epilogue: each wave turns 32 rows at a time in its own part of the LDS, so that neighbouring lanes hold neighbouring
+    // columns of a row when the residual and the pre-activation are read and the results written.
+    __syncthreads();
+    float *turn = reinterpret_cast<float *>(lds) + wave * 32 * EP_LD;
+    constexpr int LPR = FN / 4, RPP = WAVE / LPR;          // lanes per row, rows per pass
+    const int col = (lane % LPR) * 4;
+    const uint64_t n = n0 + wn + col;
+    const int ncol = n < g.N ? (int)(g.N - n < 4 ? g.N - n : 4) : 0;
+    f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+    if (P == FWD && g.bias && ncol) bias = load4_typed(g.bias, OPAL_F32, n, ncol);
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                *reinterpret_cast<f32x4 *>(turn + (lane & 31) * EP_LD + j * 32 + q * 8 + (lane >> 5) * 4) =
+                    f32x4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
+        wave_order();
+        for (int p = 0; p < 32 / RPP; p++) {
+            const int r = p * RPP + lane / LPR;
+            const uint64_t m = m0 + wm + i * 32 + r;
+            f32x4 v = *reinterpret_cast<const f32x4 *>(turn + r * EP_LD + col);
+            if (m >= g.M || !ncol) continue;
+            if constexpr (P == FWD) {
+                v += bias;
+                if (g.pre_out) store4_typed(g.pre_out, __is_same(T, float) ? OPAL_F32 : __is_same(T, f16_t) ? OPAL_F16 : OPAL_BF16, m * g.ldp + n, ncol, v);
+                if (g.act)
+                    for (int e = 0; e < 4; e++) v[e] = act_value(v[e], g.act);
+            }
+            if constexpr (P == GIN) {
+                if (g.act) {
+                    const f32x4 z = load4_typed(g.pre_in, __is_same(T, float) ? OPAL_F32 : __is_same(T, f16_t) ? OPAL_F16 : OPAL_BF16, m * g.ldp + n, ncol);
+                    for (int e = 0; e < 4; e++) v[e] *= act_slope(z[e], g.act);
+                }
+            }
+            if (P != GWT && g.res) v += load4_typed(g.res, g.res_type, m * g.ldr + n, ncol);
+            store4_typed(g.y, g.y_type, split * g.y_split + m * g.ldy + n, ncol, v);
+        }
+        wave_order();
+    }
+}
+
+// The launch of one product in one element type (opal_linear_{f32,f16,bf16}.hip); tile: 0 = 64 x 64, 1 = 128 x 128, 2 = 256 x 256
+// (16-bit types on the aligned path only).
+template <class T> hipError_t launch_linear(const Linear &g, int product, int tile, bool dma, hipStream_t stream);
+
+#define OPAL_LINEAR_CASE(T, P, TILE, BM, BN, WM, WN, D)                                                                              \
+    if (product == P && tile == TILE && dma == D) {                                                                                  \
+        hipLaunchKernelGGL((linear_kernel<T, P, BM, BN, WM, WN, D>), dim3(g.tm * g.tn * g.splits), dim3(WM * WN * WAVE), 0, stream, g); \
+        return hipGetLastError();                                                                                                    \
+    }
+#define OPAL_LINEAR_CASES(T, P)                       \
+    OPAL_LINEAR_CASE(T, P, 0, 64, 64, 2, 2, true)     \
+    OPAL_LINEAR_CASE(T, P, 0, 64, 64, 2, 2, false)    \
+    OPAL_LINEAR_CASE(T, P, 1, 128, 128, 2, 2, true)   \
+    OPAL_LINEAR_CASE(T, P, 1, 128, 128, 2, 2, false)
+
+}  // namespace opal_head

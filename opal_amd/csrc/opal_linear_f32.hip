@@ -1,0 +1,12 @@
+// The matrix products of the score head for elements of type float (opal_linear.h).
+#include "opal_linear.h"
+
+namespace opal_head {
+template <> hipError_t launch_linear<float>(const Linear &g, int product, int tile, bool dma, hipStream_t stream)
+{
+    OPAL_LINEAR_CASES(float, FWD)
+    OPAL_LINEAR_CASES(float, GIN)
+    OPAL_LINEAR_CASES(float, GWT)
+    return hipErrorInvalidValue;
+}
+}  // namespace opal_head
