@@ -599,13 +599,16 @@ static hipError_t launch(const Linear &g, int type, int product, int tile, bool 
     return launch_linear<bf16_t>(g, product, tile, dma, st);
 }
 
-constexpr int TILE[] = {64, 128};
+constexpr int TILE[] = {64, 128, 256};
 
-static int pick_tile(uint64_t M, uint64_t N, int cus)
+static uint64_t tiles_of(uint64_t M, uint64_t N, int tile) { return ((M + TILE[tile] - 1) / TILE[tile]) * ((N + TILE[tile] - 1) / TILE[tile]); }
+
+// The largest tile that still gives every CU one (256 x 256: half of them, since its kernel is twice as fast): fewer bytes for the
+// same sums against idle CUs.
+static int pick_tile(uint64_t M, uint64_t N, int cus, bool big)
 {
-    for (int t = 1; t > 0; t--)
-        if (((M + TILE[t] - 1) / TILE[t]) * ((N + TILE[t] - 1) / TILE[t]) >= (uint64_t)cus) return t;
-    return 0;
+    if (big && tiles_of(M, N, 2) * 2 >= (uint64_t)cus) return 2;
+    return tiles_of(M, N, 1) >= (uint64_t)cus ? 1 : 0;
 }
 
 static void set_tiles(Linear &g, int tile)
@@ -621,12 +624,15 @@ static int run_rows(opal_ctx *ctx, const char *who, Linear &g, int type, int pro
 {
     OnDevice on(ctx->device);
     OPAL_HIP_CHECK(ctx, on.err);
-    const int tile = pick_tile(g.M, g.N, ctx->num_cus);
+    const bool dma = aligned16(g.a, g.lda, type) && aligned16(g.b, g.ldb, type);
+    const int tile = pick_tile(g.M, g.N, ctx->num_cus, dma && type != OPAL_F32);
+    if (tiles_of(g.M, g.N, tile) >= (1ull << 31)) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": too many rows times columns for one call");
     set_tiles(g, tile);
-    if ((uint64_t)g.tm * g.tn >= (1ull << 31)) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": too many rows times columns for one call");
     g.splits = 1;
     g.ksplit = g.K;
-    OPAL_HIP_CHECK(ctx, launch(g, type, product, tile, aligned16(g.a, g.lda, type) && aligned16(g.b, g.ldb, type), ctx->stream));
+    g.items = g.tm * g.tn;
+    g.blocks = std::min<uint32_t>(g.items, ctx->num_cus);
+    OPAL_HIP_CHECK(ctx, launch(g, type, product, tile, dma, ctx->stream));
     return OPAL_OK;
 }
 
@@ -680,18 +686,21 @@ extern "C" int opal_linear_grad_input(opal_ctx *ctx, const void *d_dy, uint64_t 
     return run_rows(ctx, who, g, type, GIN);
 }
 
-// Splits of the sum over the rows: one block per CU and pass of the card, none shorter than four steps.
+// Splits of the sum over the rows, none empty.  256 x 256 tiles: as many as give the 256 CUs a tile each, of at least 16 steps.
+// Smaller ones: two blocks per CU, of at least four steps.  The choice does not look at the operands' alignment, so that the workspace
+// does not depend on it; unaligned operands take 128 x 128 tiles in the same splits.
 struct Splits { int tile; uint64_t splits, rows; };
 static Splits weight_splits(uint64_t n, uint32_t in, uint32_t out, int type)
 {
     const uint64_t step = STEP_BYTES / type_bytes(type);
-    const uint64_t steps = (n + step - 1) / step;
-    const int tile = in > 64 && out > 64 ? 1 : 0;
-    const uint64_t tiles = (uint64_t)((in + TILE[tile] - 1) / TILE[tile]) * ((out + TILE[tile] - 1) / TILE[tile]);
-    uint64_t s = std::max<uint64_t>(1, std::min<uint64_t>(512 / std::max<uint64_t>(tiles, 1), steps / 4));
-    const uint64_t per = (std::max<uint64_t>(steps, 1) + s - 1) / s;
-    s = (std::max<uint64_t>(steps, 1) + per - 1) / per;                   // none empty
-    return {tile, s, per * step};
+    const uint64_t steps = std::max<uint64_t>((n + step - 1) / step, 1);
+    const uint64_t big = tiles_of(out, in, 2);
+    const bool large = type != OPAL_F32 && in > 128 && out > 128 && steps * big >= 16 * 128;
+    const int tile = large ? 2 : in > 64 && out > 64 ? 1 : 0;
+    uint64_t s = large ? std::min<uint64_t>(256 / std::min<uint64_t>(big, 256), steps / 16) : std::min<uint64_t>(512 / std::min<uint64_t>(tiles_of(out, in, tile), 512), steps / 4);
+    s = std::max<uint64_t>(s, 1);
+    const uint64_t per = (steps + s - 1) / s;
+    return {tile, (steps + per - 1) / per, per * step};
 }
 
 constexpr uint64_t COL_PARTS = 256;       // partial column sums of dy for the bias' gradient
@@ -750,11 +759,16 @@ extern "C" int opal_linear_grad_weight(opal_ctx *ctx, const void *d_dy, uint64_t
         Linear g{};
         g.a = (const char *)d_dy; g.lda = lddy; g.b = (const char *)d_x; g.ldb = ldx;
         g.M = out; g.N = in; g.K = n;
-        set_tiles(g, s.tile);
+        const bool dma = aligned16(d_dy, lddy, type) && aligned16(d_x, ldx, type);
+        const int tile = s.tile == 2 && !dma ? 1 : s.tile;
+        if (tiles_of(out, in, tile) * s.splits >= (1ull << 31)) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": in times out is too large for one call");
+        set_tiles(g, tile);
         g.splits = (uint32_t)s.splits;
+        g.items = g.tm * g.tn * g.splits;
+        g.blocks = std::min<uint32_t>(g.items, ctx->num_cus);
         g.ksplit = s.rows;
         g.y = s.splits > 1 ? part : d_dw; g.y_type = OPAL_F32; g.ldy = s.splits > 1 ? in : lddw; g.y_split = each;
-        OPAL_HIP_CHECK(ctx, launch(g, type, GWT, s.tile, aligned16(d_dy, lddy, type) && aligned16(d_x, ldx, type), ctx->stream));
+        OPAL_HIP_CHECK(ctx, launch(g, type, GWT, tile, dma, ctx->stream));
         if (s.splits > 1) {
             hipLaunchKernelGGL(sum_splits_kernel, dim3((unsigned)std::min<uint64_t>((each + BLOCK - 1) / BLOCK, 4096)), dim3(BLOCK), 0, ctx->stream, part, s.splits, each, in, d_dw, lddw);
             OPAL_HIP_CHECK(ctx, hipGetLastError());

@@ -29,18 +29,22 @@ struct Linear {
     uint64_t y_split;             // elements between two splits' outputs
     const void *pre_in; void *pre_out; uint64_t ldp;   // the element type of the product
     int act;
+    uint32_t items, blocks;       // tiles times splits, and the blocks that share them (opal_linear_big.h)
 };
 
 constexpr float GELU_A = 1.5957691216057308f, GELU_B = 0.044715f;   // 2 sqrt(2 / pi), and the cubic term of the tanh form
 
 // v_exp_f32 and v_rcp_f32 are good to 1 ulp; the argument's rounding costs |z| 2^-24 of the result
-__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896f * z)); }
+constexpr float LOG2E = 1.44269504088896f;
+__device__ __forceinline__ float sigmoid2(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z)); }      // of -z / LOG2E
+__device__ __forceinline__ float gelu_sigmoid(float v) { return sigmoid2(v * (-LOG2E * GELU_A + -LOG2E * GELU_A * GELU_B * (v * v))); }
+__device__ __forceinline__ float sigmoid(float z) { return sigmoid2(-LOG2E * z); }
 
 __device__ __forceinline__ float act_value(float v, int act)
 {
     if (act == ACT_RELU) return v > 0.f || v != v ? v : 0.f;
     if (act == ACT_SILU) return v * sigmoid(v);
-    if (act == ACT_GELU) return v * sigmoid(GELU_A * (v + GELU_B * v * v * v));
+    if (act == ACT_GELU) return v * gelu_sigmoid(v);
     return v;
 }
 
@@ -52,7 +56,7 @@ __device__ __forceinline__ float act_slope(float v, int act)
         const float p = sigmoid(v);
         return p + c * p * (1.f - p);
     }
-    const float p = sigmoid(GELU_A * (v + GELU_B * v * v * v));
+    const float p = gelu_sigmoid(v);
     return p + c * p * (1.f - p) * GELU_A * (1.f + 3.f * GELU_B * c * c);
 }
 
@@ -80,6 +84,47 @@ template <int ES, int R> __device__ __forceinline__ int swizzle_mc(int k)
     if constexpr (ES == 4) return ((k >> 2) & 1) << 3;
     else if constexpr (R * ES >= 256) return (k & 3) << 2;
     else return ((k >> 1) & 1) << 2;
+}
+
+// Transposing reads (ds_read_b64_tr_b16): 16 lanes read four lines of 16 columns, 8 bytes each, and get the four k of one column.
+// Eight of them and their wait in one block: the builtin for this read makes the compiler wait for all chunks under way first.
+// At a's and b's place (bytes) plus 0, H, K, K + H.
+__device__ __forceinline__ uint32_t lds_place(const void *p)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    return (uint32_t)(uintptr_t)(OPAL_LDS const void *)p;
+#else
+    return 0;
+#endif
+}
+template <int H, int K> __device__ __forceinline__ void read_tr8(uint32_t a, uint32_t b, uint64_t (&x)[8])
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n\t"
+                 "ds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+                 "ds_read_b64_tr_b16 %2, %8 offset:%11\n\t"
+                 "ds_read_b64_tr_b16 %3, %8 offset:%12\n\t"
+                 "ds_read_b64_tr_b16 %4, %9\n\t"
+                 "ds_read_b64_tr_b16 %5, %9 offset:%10\n\t"
+                 "ds_read_b64_tr_b16 %6, %9 offset:%11\n\t"
+                 "ds_read_b64_tr_b16 %7, %9 offset:%12\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]), "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+                 : "v"(a), "v"(b), "n"(H), "n"(K), "n"(K + H)
+                 : "memory");
+#endif
+}
+__device__ __forceinline__ s16x8 join_tr(uint64_t lo, uint64_t hi)
+{
+    struct { uint64_t a, b; } v = {lo, hi};
+    return __builtin_bit_cast(s16x8, v);
+}
+
+// where this lane's first transposing read of the 32 columns from r0 on begins, in an MC tile of R columns
+template <int R> __device__ __forceinline__ uint32_t tr_place(int r0)
+{
+    const int lane = threadIdx.x & 63, col = r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4, k = (lane >> 5) * 8 + ((lane >> 2) & 3);
+    return (uint32_t)(k * (R * 2) + (((col >> 3) ^ swizzle_mc<2, R>(k)) * 16) + (col & 7) * 2);
 }
 
 // One operand's tile: R rows (m or n) of one step of k.
@@ -167,28 +212,20 @@ template <class T, int R, bool KC, int NT, bool DMA> struct Operand {
         }
     }
 
-    // Fragment of 32 rows from r0 on, 16-bit types: k = 16 kk + 8 (lane / 32) + 0..7 of row r0 + lane % 32.
-    __device__ __forceinline__ static s16x8 frag16(const char *lds, int r0, int kk)
+    // Fragments of 32 rows from r0 on and a step's four times 16 k, 16-bit types: k = 16 kk + 8 (lane / 32) + 0..7 of row r0 + lane % 32.
+    __device__ __forceinline__ static void frag16(const char *lds, int r0, s16x8 (&f)[4])
     {
         const int lane = threadIdx.x & 63;
         if constexpr (KC) {
-            const int r = r0 + (lane & 31), c = kk * 2 + (lane >> 5);
-            return *reinterpret_cast<const s16x8 *>(lds + r * STEP_BYTES + ((c ^ swizzle_kc(r)) * 16));
+            const int r = r0 + (lane & 31);
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) f[kk] = *reinterpret_cast<const s16x8 *>(lds + r * STEP_BYTES + (((kk * 2 + (lane >> 5)) ^ swizzle_kc(r)) * 16));
         } else {
-            s16x8 v = {};
-#ifdef __HIP_DEVICE_COMPILE__
-            // 16 lanes read four lines of 16 columns, 8 bytes each, and get the four k of one column
-            const int col = r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+            const uint32_t a = lds_place(lds) + tr_place<R>(r0);
+            uint64_t x[8];
+            read_tr8<4 * R * 2, 16 * R * 2>(a, a + 32 * R * 2, x);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int k = kk * 16 + (lane >> 5) * 8 + h * 4 + ((lane >> 2) & 3);
-                const char *p = lds + k * (R * ES) + (((col >> 3) ^ swizzle_mc<ES, R>(k)) * 16) + (col & 7) * 2;
-                const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((OPAL_LDS s16x4 *)p);
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[h * 4 + e] = t[e];
-            }
-#endif
-            return v;
+            for (int kk = 0; kk < 4; kk++) f[kk] = join_tr(x[2 * kk], x[2 * kk + 1]);
         }
     }
     // 32-bit type: k = 8 j + 4 (lane / 32) + 0..3 of row r0 + lane % 32.
@@ -286,18 +323,17 @@ __global__ __launch_bounds__(WM * WN * WAVE) void linear_kernel(const Linear g)
         }
         const char *la = cur, *lb = cur + BM * STEP_BYTES;
         if constexpr (ES == 2) {
+            s16x8 fa[TM][4], fb[TN][4];
 #pragma unroll
-            for (int kk = 0; kk < STEP / 16; kk++) {
-                s16x8 fa[TM], fb[TN];
+            for (int i = 0; i < TM; i++) OA::frag16(la, wm + i * 32, fa[i]);
 #pragma unroll
-                for (int i = 0; i < TM; i++) fa[i] = OA::frag16(la, wm + i * 32, kk);
+            for (int j = 0; j < TN; j++) OB::frag16(lb, wn + j * 32, fb[j]);
 #pragma unroll
-                for (int j = 0; j < TN; j++) fb[j] = OB::frag16(lb, wn + j * 32, kk);
+            for (int kk = 0; kk < 4; kk++)
 #pragma unroll
                 for (int i = 0; i < TM; i++)
 #pragma unroll
-                    for (int j = 0; j < TN; j++) acc[i][j] = mfma16<T>(fb[j], fa[i], acc[i][j]);
-            }
+                    for (int j = 0; j < TN; j++) acc[i][j] = mfma16<T>(fb[j][kk], fa[i][kk], acc[i][j]);
         } else {
 #pragma unroll
             for (int kk = 0; kk < STEP / 8; kk++) {

@@ -1,0 +1,549 @@
+// The product kernel for large 16-bit matrices on 16 bytes (opal_linear.h has the products, the operands' layouts and the kernel
+// for everything else): 256 x 256 tiles, eight waves of 128 x 64, one block per CU that stays for all its tiles, steps of 32 k.
+//
+// What bounds it is the matrix pipe, so everything else runs beside it.
+//   - Waves 0 .. 3 and 4 .. 7 share the four SIMDs and take turns: while one half multiplies (16 MFMAs, its requests for chunks in
+//     between), the other reads its next fragments, with a barrier at each change; half 1 runs one change behind half 0.
+//   - Chunks come straight into LDS, well ahead and over the ends of tiles.  Half 0 asks for A's, half 1 for B's: vmcnt counts a
+//     wave's requests in their order, so A's long way (memory) and B's short one (W stays in L2) must not share a count.
+//   - A of FWD and GIN is fetched 64 k at a time: whole 128-byte lines, of which a CU has only so many on their way.
+//   - The epilogue works in the accumulators' own places; its stores drain under the next tile's steps.
+#pragma once
+#include "opal_linear.h"
+
+namespace opal_head {
+
+// Four neighbouring elements of a matrix whose type is known at run time, as they lie in memory: loads can be started well
+// before they are used.
+struct RawQuad { uint32_t w[4]; };
+__device__ __forceinline__ RawQuad load_raw(const void *base, int type, uint64_t at, int m)
+{
+    RawQuad r = {{0, 0, 0, 0}};
+    if (m >= 4) {
+        if (type == OPAL_F32) {
+            const Quad<float> q = *reinterpret_cast<const Quad<float> *>((const float *)base + at);
+            __builtin_memcpy(r.w, &q, 16);
+        } else {
+            const Quad<f16_t> q = *reinterpret_cast<const Quad<f16_t> *>((const f16_t *)base + at);
+            __builtin_memcpy(r.w, &q, 8);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+            if (i < m) {
+                if (type == OPAL_F32) r.w[i] = ((const uint32_t *)base)[at + i];
+                else r.w[i / 2] |= (uint32_t)((const uint16_t *)base)[at + i] << (16 * (i & 1));
+            }
+    }
+    return r;
+}
+__device__ __forceinline__ f32x4 decode(const RawQuad &r, int type)
+{
+    if (type == OPAL_F32) return f32x4{__builtin_bit_cast(float, r.w[0]), __builtin_bit_cast(float, r.w[1]), __builtin_bit_cast(float, r.w[2]), __builtin_bit_cast(float, r.w[3])};
+    if (type == OPAL_BF16)
+        return f32x4{__builtin_bit_cast(float, r.w[0] << 16), __builtin_bit_cast(float, r.w[0] & 0xffff0000u), __builtin_bit_cast(float, r.w[1] << 16),
+                     __builtin_bit_cast(float, r.w[1] & 0xffff0000u)};
+    struct H { f16_t v[4]; };
+    H h;
+    __builtin_memcpy(&h, r.w, 8);
+    return f32x4{(float)h.v[0], (float)h.v[1], (float)h.v[2], (float)h.v[3]};
+}
+
+constexpr int BIG = 256, BIG_THREADS = 512, BIG_STEP = 32;
+
+// k per stage and stages of an operand's ring.  FWD, GIN: A 3 x 64 k (96 KB), B 3 x 32 k (48 KB); GWT, whose operands both come
+// from memory in whole lines (MC): 4 x 32 k each (128 KB).  Each of a half's four waves asks for four chunks a lane and step.
+//
+// When a stage's place is free: both halves have read stage s once half 1 multiplies it (it reads after half 0), which is when half 1
+// asks for B's stage s + N; half 0, which asks for A, multiplies one change earlier and may only refill the place of the stage before:
+// A's stage s + N - 1.
+template <int P, bool IS_A> struct Ring {
+    static constexpr bool KC = IS_A ? P != GWT : P == FWD;
+    static constexpr int K = P != GWT && IS_A ? 64 : 32, N = P == GWT ? 4 : 3;
+    static constexpr int BYTES = BIG * K * 2, PARTS = K / BIG_STEP, AHEAD = IS_A ? N - 1 : N;
+    static constexpr int WAIT = (N - 2) * 4 * PARTS;                          // requests that may be on their way behind the next stage's
+    static constexpr int LINE = KC ? K / 8 : 32;                              // chunks: KC has 256 lines, MC one for each k
+    // KC: lines of 128 (64) bytes, two (four) of which share the banks: the rotation gives a chunk of 16 rows 16 places
+    __device__ __forceinline__ static int swz(int line) { return !KC ? swizzle_mc<2, BIG>(line) : K == 64 ? swizzle_kc(line) : (line >> 2) & 3; }
+    // bytes from a stage's first element on that are the matrix's, up to the end of the 16 that hold the last one; lines behind read as zeros
+    __device__ __forceinline__ static uint32_t length(uint32_t ld, int rows, int kval)
+    {
+        return ((uint32_t)((KC ? rows : kval) - 1) * ld + (uint32_t)(KC ? kval : rows) * 2u + 15u) & ~15u;
+    }
+    // Fragments of COUNT times 32 rows from r0 on and of the 32 k that begin at 16 kk: k = 8 (lane / 32) + 0..7 of 16.
+    template <int COUNT> __device__ __forceinline__ static void frags(const char *lds, int r0, int kk, s16x8 (&f)[2][COUNT])
+    {
+        const int lane = threadIdx.x & 63;
+        if constexpr (KC) {
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int i = 0; i < COUNT; i++) {
+                    const int r = r0 + i * 32 + (lane & 31), c = (kk + s) * 2 + (lane >> 5);
+                    f[s][i] = *reinterpret_cast<const s16x8 *>(lds + r * (K * 2) + ((c ^ swz(r)) * 16));
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < COUNT; i += 2) {
+                uint64_t x[8];
+                read_tr8<4 * BIG * 2, 16 * BIG * 2>(lds_place(lds) + tr_place<BIG>(r0 + i * 32), lds_place(lds) + tr_place<BIG>(r0 + i * 32 + 32), x);
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    f[s][i] = join_tr(x[2 * s], x[2 * s + 1]);
+                    f[s][i + 1] = join_tr(x[4 + 2 * s], x[5 + 2 * s]);
+                }
+            }
+        }
+    }
+};
+constexpr int BIG_TURN = 8 * 64 * 4;           // bytes: a wave's turning place
+
+// the k of a KC fragment behind the matrix's edge: `left` values of k from the fragment's first on are the matrix's
+__device__ __forceinline__ s16x8 keep_k(s16x8 f, int left)
+{
+    u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = left >= 2 * i + 2 ? w[i] : left == 2 * i + 1 ? w[i] & 0xffffu : 0u;
+    return __builtin_bit_cast(s16x8, w);
+}
+
+struct BigItem {                               // one tile (of one split)
+    uint32_t m0, n0, split;
+    int rows_a, rows_b;
+    uint64_t k, count;                         // first k, number of k
+};
+template <int P> __device__ __forceinline__ BigItem big_item(const Linear &g, uint32_t i)
+{
+    uint32_t t = xcd_tile(i, g.items);
+    const uint32_t tiles = g.tm * g.tn, split = P == GWT ? t / tiles : 0;
+    t -= split * tiles;
+    BigItem r;
+    const uint32_t tm = t / g.tn, tn = t - tm * g.tn;
+    r.m0 = tm * BIG;
+    r.n0 = tn * BIG;
+    r.split = split;
+    r.rows_a = (int)(g.M - r.m0 < (uint64_t)BIG ? g.M - r.m0 : (uint64_t)BIG);
+    r.rows_b = (int)(g.N - r.n0 < (uint64_t)BIG ? g.N - r.n0 : (uint64_t)BIG);
+    r.k = split * g.ksplit;
+    r.count = (P == GWT && r.k + g.ksplit < g.K ? r.k + g.ksplit : g.K) - r.k;
+    return r;
+}
+
+// The launch's description, read again from the argument segment (a few hundred cycles, once a tile) rather than kept in scalar
+// registers through the loop, where there are none to spare.
+__device__ __forceinline__ const Linear &reload()
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    auto p = (const __attribute__((address_space(4))) Linear *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Linear *)p;
+#else
+    __builtin_unreachable();
+#endif
+}
+
+// A wave's requests: half 0 feeds A, half 1 B.  The two differ in numbers only, so that a request is the same instruction for both.
+template <int P> struct Feed {
+    using RA = Ring<P, true>;
+    using RB = Ring<P, false>;
+    const char *p;                             // the next stage's first element
+    uint64_t step;
+    uint32_t off, hop, ring, item, slot, left, len, last;
+    uint32_t at, now, to;                      // of the requests at hand
+    int lim, tail, half;                       // lim: first k of this thread's chunks (KC), -1 where the end of k cuts lines (MC)
+
+    __device__ __forceinline__ void init(int wave)
+    {
+        const Linear &g = reload();
+        half = wave >> 2;
+        const uint32_t t = threadIdx.x & 255;
+        place<RA>(g.lda, half == 0, t);
+        place<RB>(g.ldb, half == 1, t);
+        ring = (half ? RA::N * RA::BYTES : 0) + (wave & 3) * 1024;
+        item = blockIdx.x;
+        slot = 0;
+        open();
+    }
+    template <class R> __device__ __forceinline__ void place(uint64_t elements, bool mine, uint32_t t)
+    {
+        static_assert((256 / R::LINE) % 16 == 0 || !R::KC, "the rotation repeats after 16 lines");
+        if (!mine) return;
+        const uint32_t ld = (uint32_t)elements * 2, line = t / R::LINE, chunk = (t % R::LINE) ^ R::swz(line);
+        off = line * ld + chunk * 16;
+        hop = 256 / R::LINE * ld;              // whole rotations further: the same place in the line
+        lim = R::KC ? (int)chunk * 8 : -1;
+        step = R::KC ? R::K * 2 : (uint64_t)R::K * ld;
+    }
+    // Turns to the tile `item`; behind the last one to an empty buffer (zeros that nobody reads): every stage has the same requests.
+    __device__ __forceinline__ void open()
+    {
+        const Linear &g = reload();
+        const bool any = item < g.items;
+        const BigItem f = big_item<P>(g, any ? item : 0);
+        if (half == 0) aim<RA>(g.a, g.lda * 2, f.m0, f.rows_a, f, any);
+        else aim<RB>(g.b, g.ldb * 2, f.n0, f.rows_b, f, any);
+    }
+    template <class R> __device__ __forceinline__ void aim(const char *matrix, uint64_t ld, uint64_t first, int rows, const BigItem &f, bool any)
+    {
+        const uint32_t stages = (uint32_t)((f.count + R::K - 1) / R::K);
+        p = matrix + (R::KC ? first * ld + f.k * 2 : f.k * ld + first * 2);
+        tail = any ? (int)(f.count - (uint64_t)(stages - 1) * R::K) : R::K;
+        left = any ? stages : 0x7fffffffu;
+        len = any ? R::length((uint32_t)ld, rows, R::K) : 0;
+        last = any ? R::length((uint32_t)ld, rows, tail) : 0;
+    }
+    // the requests of a step: `part` of the stage, 0 .. PARTS - 1
+    __device__ __forceinline__ void start(int part)
+    {
+        at = left == 1 && lim >= tail ? 0x80000000u : off;       // behind every buffer (smaller than 2^31)
+        at += part * 4 * hop;
+        now = left == 1 ? last : len;
+        to = ring + slot * (half ? RB::BYTES : RA::BYTES) + part * 4 * 4096;
+    }
+    __device__ __forceinline__ void request(char *lds, int i) const
+    {
+#ifdef __HIP_DEVICE_COMPILE__
+        auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, (int)now, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (OPAL_LDS void *)(lds + to + i * 4096), 16, (int)(at + i * hop), 0, 0, 0);
+#endif
+    }
+    __device__ __forceinline__ void done()     // the stage is asked for
+    {
+        slot = slot + 1 == (uint32_t)RA::N ? 0 : slot + 1;
+        p += step;
+        if (--left == 0) {
+            item += reload().blocks;
+            open();
+        }
+    }
+    __device__ __forceinline__ void stage(char *lds)
+    {
+        for (int part = 0; part < (half ? RB::PARTS : RA::PARTS); part++) {
+            start(part);
+            for (int i = 0; i < 4; i++) request(lds, i);
+        }
+        done();
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ epilogue
+template <class T> __device__ __forceinline__ constexpr int own_type() { return __is_same(T, f16_t) ? OPAL_F16 : OPAL_BF16; }
+
+// Tiles at the edge of N that cut a group of eight columns, and the rarer mixes of types: the wave's 128 x 64 results, eight rows at
+// a time (slice = 4 i + quarter) through its own 2 KB of LDS, one element after the other: little code, since what a tile executes
+// has to stay in the instruction cache.
+__device__ __forceinline__ float load1(const void *base, int type, uint64_t at)
+{
+    return type == OPAL_F32 ? ((const float *)base)[at] : type == OPAL_F16 ? (float)((const f16_t *)base)[at] : (float)((const bf16_t *)base)[at];
+}
+__device__ __forceinline__ void store1(void *base, int type, uint64_t at, float v)
+{
+    if (type == OPAL_F32) ((float *)base)[at] = v;
+    else if (type == OPAL_F16) ((f16_t *)base)[at] = (f16_t)v;
+    else ((bf16_t *)base)[at] = (bf16_t)v;
+}
+template <class T, int P, int ACT>
+__device__ __forceinline__ void epilogue_any(const Linear &g, const BigItem &c, const f32x16 (&acc)[4][2], float *turn, int wm, int wn)
+{
+    constexpr int own = own_type<T>();
+    const int lane = threadIdx.x & 63;
+    const uint32_t n = c.n0 + wn + lane, m0 = c.m0 + wm;
+    float bias = P == FWD && g.bias && n < g.N ? g.bias[n] : 0.f;
+    asm volatile("" : "+v"(bias));             // arrives here: were it left to its use, the main loop would be made to wait for it
+#pragma unroll 1
+    for (int s = 0; s < 16; s++) {
+        const int r = lane & 7;
+        if (((lane >> 3) & 3) == (s & 3)) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if ((s >> 2) == i)
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            *reinterpret_cast<f32x4 *>(turn + r * 64 + (((j * 8 + q * 2 + (lane >> 5)) ^ (r * 2)) * 4)) =
+                                f32x4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
+        }
+        wave_order();
+#pragma unroll 2
+        for (int row = 0; row < 8; row++) {                    // a lane a column
+            const uint64_t m = m0 + s * 8 + row;
+            float v = turn[row * 64 + (((lane >> 2) ^ (row * 2)) * 4) + (lane & 3)];
+            if (m < g.M && n < g.N) {
+                if (P == GIN && ACT) v *= act_slope(load1(g.pre_in, own, m * g.ldp + n), ACT);
+                if (P == FWD) {
+                    v += bias;
+                    if (g.pre_out) store1(g.pre_out, own, m * g.ldp + n, v);
+                    v = act_value(v, ACT);
+                }
+                if (P != GWT && g.res) v += load1(g.res, g.res_type, m * g.ldr + n);
+                store1(g.y, g.y_type, c.split * g.y_split + m * g.ldy + n, v);
+            }
+        }
+        wave_order();
+    }
+}
+
+// Eight columns of a row in a 16-bit type, 16 bytes: the lanes l and l + 32 hold columns 0..3 and 4..7 of the groups x and y (of the
+// same row); afterwards l holds the eight of x and l + 32 those of y.
+__device__ __forceinline__ u32x4 join_halves(uint32_t x0, uint32_t x1, uint32_t y0, uint32_t y1)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    const auto a = __builtin_amdgcn_permlane32_swap(x0, y0, false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(x1, y1, false, false);
+    return u32x4{a[0], b[0], a[1], b[1]};
+#else
+    return u32x4{x0, x1, y0, y1};
+#endif
+}
+template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    struct H { T v[2]; } h = {{(T)a, (T)b}};
+    return __builtin_bit_cast(uint32_t, h);
+}
+struct __attribute__((packed, aligned(2))) Any16 { uint32_t w[4]; };
+struct __attribute__((packed, aligned(2))) Any8 { uint32_t w[2]; };
+
+// Whole groups of eight columns, results in 32 bits or the operands' type: 32 x 32 results at a time, straight from the accumulators.
+// A lane holds row l % 32 and, of a group of eight columns, four; 16-bit results are joined to 16 bytes a lane.  What is read is
+// asked for one block ahead.
+template <class T> __device__ __forceinline__ void store_joined(void *to, uint64_t at, bool in, const f32x16 &a, int qq)
+{
+    const u32x4 o = join_halves(pack2<T>(a[qq * 8], a[qq * 8 + 1]), pack2<T>(a[qq * 8 + 2], a[qq * 8 + 3]), pack2<T>(a[qq * 8 + 4], a[qq * 8 + 5]),
+                                pack2<T>(a[qq * 8 + 6], a[qq * 8 + 7]));
+    if (in) *reinterpret_cast<Any16 *>((T *)to + at) = __builtin_bit_cast(Any16, o);
+}
+
+template <class T, int P, int ACT, bool Y32, bool RES>
+__device__ __forceinline__ void epilogue_plain(const Linear &g, const BigItem &c, const f32x16 (&acc)[4][2], int wm, int wn)
+{
+    constexpr int own = own_type<T>();
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const uint32_t m0 = c.m0 + wm + (lane & 31), n0 = c.n0 + wn, N = (uint32_t)g.N, M = (uint32_t)g.M;
+    const uint32_t nq = n0 + h * 4, nj = n0 + h * 8;           // this lane's columns of a group, and of two groups joined
+    constexpr bool with_res = RES, with_pre = P == GIN && ACT;      // known here: a load that might not be used would be waited for in the loop
+    RawQuad res[2][4], pre[2][4];
+    auto ask = [&](int t) __attribute__((always_inline)) {
+        const uint32_t m = m0 + (t >> 1) * 32;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const uint32_t n = nq + (t & 1) * 32 + q * 8;
+            const int w = m < M && n < N ? 4 : 0;
+            if (with_res) res[t & 1][q] = load_raw(g.res, g.res_type, m * g.ldr + n, w);
+            if (with_pre) pre[t & 1][q] = load_raw(g.pre_in, own, m * g.ldp + n, w);
+        }
+    };
+    if (with_res || with_pre) ask(0);
+    f32x4 bias[2][4] = {};
+    if (P == FWD && g.bias)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                if (nq + j * 32 + q * 8 < N) bias[j][q] = load4(g.bias + nq + j * 32 + q * 8);
+#pragma unroll
+    for (int t = 0; t < 8; t++) {
+        const uint32_t m = m0 + (t >> 1) * 32;
+        f32x16 v = acc[t >> 1][t & 1];
+        if ((with_res || with_pre) && t < 7) ask(t + 1);
+        if (P == FWD) {
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[q * 4 + e] += bias[t & 1][q][e];
+        }
+        if (P == FWD && g.pre_out) {
+#pragma unroll
+            for (int qq = 0; qq < 2; qq++) {
+                const uint32_t n = nj + (t & 1) * 32 + qq * 16;
+                store_joined<T>(g.pre_out, m * g.ldp + n, m < M && n < N, v, qq);
+            }
+        }
+        if (P == FWD && ACT) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) v[e] = act_value(v[e], ACT);
+        }
+        if (with_pre) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const f32x4 z = decode(pre[t & 1][q], own);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[q * 4 + e] *= act_slope(z[e], ACT);
+            }
+        }
+        if (with_res) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const f32x4 r = decode(res[t & 1][q], g.res_type);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[q * 4 + e] += r[e];
+            }
+        }
+        if constexpr (Y32) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const uint32_t n = nq + (t & 1) * 32 + q * 8;
+                if (m < M && n < N) store4((float *)g.y + c.split * g.y_split + m * g.ldy + n, f32x4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]});
+            }
+        } else {
+#pragma unroll
+            for (int qq = 0; qq < 2; qq++) {
+                const uint32_t n = nj + (t & 1) * 32 + qq * 16;
+                store_joined<T>(g.y, m * g.ldy + n, m < M && n < N, v, qq);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ main loop
+// One step of a wave: fragments, the change of turns, 16 MFMAs and its requests.  CUT: the last step of a sum whose k end inside a
+// chunk.  sub: the step's 32 k within A's stage.  fresh: the next step begins a new stage of A; last: of the tile.
+template <class T, int P, bool CUT>
+__device__ __forceinline__ void big_step(Feed<P> &feed, f32x16 (&acc)[4][2], char *lds, uint32_t slot_a, uint32_t slot_b, int sub, bool fresh, bool last, int wave,
+                                         int half, int &landed, int ctail)
+{
+    using RA = Ring<P, true>;
+    using RB = Ring<P, false>;
+    const char *sa = lds + slot_a * RA::BYTES, *sb = lds + RA::N * RA::BYTES + slot_b * RB::BYTES;
+    const int wm = half * 128, wn = (wave & 3) * 64;
+    s16x8 fa[2][4], fb[2][2];
+    RA::template frags<4>(sa, wm, sub * 2, fa);
+    RB::template frags<2>(sb, wn, 0, fb);
+    if constexpr (CUT) {
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            const int left = ctail - kk * 16 - ((threadIdx.x >> 5) & 1) * 8;
+#pragma unroll
+            for (int i = 0; i < 4; i++) fa[kk][i] = keep_k(fa[kk][i], left);
+            if (P == FWD)
+#pragma unroll
+                for (int j = 0; j < 2; j++) fb[kk][j] = keep_k(fb[kk][j], left);
+        }
+    }
+    const int part = half ? 0 : sub;
+    feed.start(part);
+    // The next stage has to be there before the barrier that opens it for half 0: half 1's requests here, half 0's behind its MFMAs.
+    // vmcnt counts stores too, which an epilogue leaves behind; it waits for what was asked for before it, so that the next stages
+    // need not wait for its stores (landed).
+    if (half) {
+        if (landed > 0) landed--;
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(RB::WAIT) : "memory");
+    }
+    // Between the two barriers of a turn stands nothing but MFMAs and, in their shadow, the requests (one for four of them).
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) acc[i][j] = mfma16<T>(fb[kk][j], fa[kk][i], acc[i][j]);
+            if ((i & 1) == 0) {
+                __builtin_amdgcn_sched_barrier(0);
+                feed.request(lds, kk * 2 + i / 2);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!half) {
+        if (fresh) {
+            if (sub < RA::PARTS - 1) {         // a tile that ends inside a stage: the rest of the requests
+                feed.start(sub + 1);
+                for (int i = 0; i < 4; i++) feed.request(lds, i);
+            }
+            if (landed > 0) landed--;
+            else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(RA::WAIT) : "memory");
+        }
+        asm volatile("s_barrier" ::: "memory");
+        if (fresh) feed.done();
+    } else {
+        if (!last) asm volatile("s_barrier" ::: "memory");     // of a tile: behind the epilogue
+        feed.done();
+    }
+}
+
+template <class T, int P, int ACT, bool Y32, bool RES> __global__ __launch_bounds__(BIG_THREADS, 1) void linear_big_kernel(const Linear)
+{
+    using RA = Ring<P, true>;
+    using RB = Ring<P, false>;
+    static_assert(RA::N == RB::N && RA::PARTS <= 2, "");
+    __shared__ __attribute__((aligned(128))) char lds[RA::N * RA::BYTES + RB::N * RB::BYTES + 8 * BIG_TURN];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave >> 2;
+    Feed<P> feed;
+    feed.init(wave);
+    const int ahead = half ? RB::AHEAD : RA::AHEAD;
+#pragma unroll 1
+    for (int i = 0; i < ahead; i++) feed.stage(lds);
+    int landed = ahead - 1;                    // stages behind the current one that are known to be in LDS
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    uint32_t ci = blockIdx.x, slot_a = 0, slot_b = 0;
+    if (half) asm volatile("s_barrier" ::: "memory");
+    while (true) {
+        f32x16 acc[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+        const uint64_t count = big_item<P>(reload(), ci).count;
+        const uint32_t steps = (uint32_t)((count + BIG_STEP - 1) / BIG_STEP);
+        const int tail = (int)(count - (uint64_t)(steps - 1) * BIG_STEP);
+        const bool odd = P != GWT && (tail & 7);
+        const uint32_t whole = odd ? steps - 1 : steps;
+        int sub = 0;
+#pragma unroll 1
+        for (uint32_t s = 0; s < whole; s++) {
+            const bool fresh = sub == RA::PARTS - 1 || s + 1 == steps;
+            big_step<T, P, false>(feed, acc, lds, slot_a, slot_b, sub, fresh, s + 1 == steps, wave, half, landed, 0);
+            slot_b = slot_b + 1 == RB::N ? 0 : slot_b + 1;
+            if (fresh) slot_a = slot_a + 1 == RA::N ? 0 : slot_a + 1;
+            sub = fresh ? 0 : sub + 1;
+        }
+        if (odd) {
+            big_step<T, P, true>(feed, acc, lds, slot_a, slot_b, sub, true, true, wave, half, landed, tail);
+            slot_b = slot_b + 1 == RB::N ? 0 : slot_b + 1;
+            slot_a = slot_a + 1 == RA::N ? 0 : slot_a + 1;
+        }
+        // the two halves' epilogues fall into the same change: half 0's behind its barrier, half 1's ahead of it
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        landed = ahead - 1;
+        const Linear &g = reload();
+        const BigItem c = big_item<P>(g, ci);
+        constexpr int own = own_type<T>();
+        const bool plain = (g.N - c.n0 >= BIG || g.N % 8 == 0) && g.y_type == (Y32 ? OPAL_F32 : own) && (!RES || g.res_type == OPAL_F32 || g.res_type == own);
+        if (plain) epilogue_plain<T, P, ACT, Y32, RES>(g, c, acc, half * 128, (wave & 3) * 64);
+        else epilogue_any<T, P, ACT>(g, c, acc, reinterpret_cast<float *>(lds + RA::N * RA::BYTES + RB::N * RB::BYTES + wave * BIG_TURN), half * 128, (wave & 3) * 64);
+        ci += g.blocks;
+        if (ci >= g.items) break;
+        if (half) asm volatile("s_barrier" ::: "memory");
+    }
+    // what was asked for behind the end was waited for above: nothing arrives in LDS that is another block's by then
+}
+
+// One kernel for each activation and width of the result: what a tile executes has to stay in the instruction cache.
+template <class T> hipError_t launch_big(const Linear &g, int product, hipStream_t stream)
+{
+#define OPAL_BIG(P, ACT, Y32, RES)                                                                                          \
+    if (product == P && (P == GWT || (g.act == ACT && (g.y_type == OPAL_F32) == Y32 && (g.res != nullptr) == RES))) {        \
+        hipLaunchKernelGGL((linear_big_kernel<T, P, ACT, Y32, RES>), dim3(g.blocks), dim3(BIG_THREADS), 0, stream, g);       \
+        return hipGetLastError();                                                                                           \
+    }
+#define OPAL_BIGS2(P, Y32, RES) \
+    OPAL_BIG(P, ACT_NONE, Y32, RES) OPAL_BIG(P, ACT_RELU, Y32, RES) OPAL_BIG(P, ACT_SILU, Y32, RES) OPAL_BIG(P, ACT_GELU, Y32, RES)
+#define OPAL_BIGS(P, Y32) OPAL_BIGS2(P, Y32, false) OPAL_BIGS2(P, Y32, true)
+    OPAL_BIGS(FWD, false)
+    OPAL_BIGS(FWD, true)
+    OPAL_BIGS(GIN, false)
+    OPAL_BIGS(GIN, true)
+    OPAL_BIG(GWT, ACT_NONE, true, false)
+#undef OPAL_BIGS
+#undef OPAL_BIGS2
+#undef OPAL_BIG
+    return hipErrorInvalidValue;
+}
+
+}  // namespace opal_head

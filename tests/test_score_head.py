@@ -136,6 +136,72 @@ def test_linear_gradients(eng, t, n, k, m, pad):
     assert none is None and torch.equal(dw, dw2)
 
 
+# enough rows and columns for the 256 x 256 tiles of 16-bit products: sums that end inside a step, a chunk, a stage of 64; columns that
+# end inside a group of eight; several tiles a block; every epilogue
+BIG_SHAPES = [(16700, 100, 520), (33000, 71, 250), (11000, 40, 1563), (16500, 1, 512), (8200, 355, 1030), (70001, 33, 257), (16400, 192, 511), (9000, 1563, 1040)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("n,k,m", BIG_SHAPES)
+@pytest.mark.parametrize("out", [F32, None, "other"])
+def test_large_products(eng, t, n, k, m, out):
+    """A thousand rows of the result, the first and the last ones among them, and its gradients."""
+    g = torch.Generator(device="cuda").manual_seed(n + k + m)
+    rnd = lambda a, b, s=1.0: (torch.randn(a, -(-b // 8) * 8, device="cuda", generator=g) * s).to(t)[:, :b]  # noqa: E731
+    x, w, dy, pre = rnd(n, k), rnd(m, k, k ** -0.5), rnd(n, m, 0.1), rnd(n, k)
+    out = {None: t, "other": F16 if t == BF16 else BF16}.get(out, out)
+    act = ["none", "relu", "silu", "gelu"][(n + m + (out == F32)) % 4]
+    bias = torch.randn(m, device="cuda", generator=g) if m % 2 == 0 else None
+    res = rnd(n, m).to([F32, t, out][n % 3]) if k % 2 else None
+    at = torch.cat([torch.arange(300), torch.randint(0, n, (400,), generator=gen("rows")), torch.arange(n - 300, n)])
+    y, saved = eng.linear(x, w, bias, activation=act, residual=res, out_dtype=out, want_pre=True)
+    x64, w64 = x[at.cuda()].double().cpu(), w.double().cpu()
+    p = x64 @ w64.t()
+    dp = (k + 3) * U * (x64.abs() @ w64.abs().t())
+    if bias is not None:
+        p, dp = p + bias.double().cpu(), dp + (k + 3) * U * bias.double().abs().cpu()
+    close(saved[at.cuda()], p, dp + rounding(p.abs() + dp, t), "pre")
+    a = act64(p, act)
+    da = 1.13 * dp + U * (8 + 4 * p.abs() + 2 * p.abs() ** 3) * a.abs() + 1e-37
+    ref = a + (res[at.cuda()].double().cpu() if res is not None else 0.0)
+    d = da + U * (ref.abs() + a.abs() + da)
+    close(y[at.cuda()], ref, d + rounding(ref.abs() + d, out), "y")
+    assert torch.isfinite(y.float()).all()
+    res = rnd(n, k).to([F32, t, out][n % 3]) if m % 2 else None
+    dx = eng.linear_grad_input(dy, w, pre=pre if act != "none" else None, activation=act, residual=res, out_dtype=out)
+    dy64, pre64 = dy[at.cuda()].double().cpu(), pre[at.cuda()].double().cpu()
+    s = slope64(pre64, act)
+    p = dy64 @ w64
+    d = s.abs() * (m + 2) * U * (dy64.abs() @ w64.abs())
+    ds = U * (16 + 16 * pre64.abs() + 8 * pre64.abs() ** 3) if act in ("silu", "gelu") else 0.0
+    ref = p * s + (res[at.cuda()].double().cpu() if res is not None else 0.0)
+    d = d + p.abs() * ds + 2 * U * (ref.abs() + (p * s).abs())
+    close(dx[at.cuda()], ref, d + rounding(ref.abs() + d, out), "dx")
+    assert torch.isfinite(dx.float()).all()
+    if out == F32:
+        dw, db = eng.linear_grad_weight(dy, x)
+        dy64, x64 = dy.double().cpu(), x.double().cpu()
+        close(dw, dy64.t() @ x64, (n + 2) * U * (dy64.abs().t() @ x64.abs()) + 1e-38, "dw")
+        close(db, dy64.sum(0), (n + 2) * U * dy64.abs().sum(0) + 1e-38, "db")
+
+
+@pytest.mark.gpu
+def test_large_products_keep_nans_behind_the_edge_out(eng):
+    """What lies between the rows is NaN: it must not reach a sum, also where the last chunk of a row is cut."""
+    n, k, m = 16700, 99, 515
+    for t in (F16, BF16):
+        full = [torch.full((r, c), float("nan"), device="cuda", dtype=t) for r, c in ((n, 104), (m, 112), (n, 520))]
+        x, w, dy = full[0][:, :k], full[1][:, :k], full[2][:, :m]
+        for v in (x, w, dy):
+            v.copy_(torch.randn(v.shape, device="cuda"))
+        y, _ = eng.linear(x, w, out_dtype=F32)
+        assert torch.isfinite(y).all()
+        assert torch.isfinite(eng.linear_grad_input(dy, w, out_dtype=F32)).all()
+        dw, db = eng.linear_grad_weight(dy, x)
+        assert torch.isfinite(dw).all() and torch.isfinite(db).all()
+
+
 @pytest.mark.gpu
 def test_products_of_no_rows(eng):
     w = torch.randn(5, 7, device="cuda")
