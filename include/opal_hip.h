@@ -285,7 +285,7 @@ int opal_linear_grad_input(opal_ctx *ctx, const void *d_dy, uint64_t lddy, const
                            uint64_t ldp, int activation, const void *d_res, int res_type, uint64_t ldr, uint64_t n, uint32_t in,
                            uint32_t out, void *d_dx, int dx_type, uint64_t lddx);
 
-/* dw[out, in] = dy[n, out]^T x[n, in] and dbias[out] = sum over rows of dy, in float32; either may be NULL.  dy is the gradient
+/* dw[out, in] = dy[n, out]^T x[n, in] and dbias[out] = sum over rows of dy (NULL = not wanted), in float32.  dy is the gradient
  * before the activation.  d_work: opal_linear_grad_weight_workspace(n, in, out, type) bytes (OPAL_ERANGE when smaller).  */
 uint64_t opal_linear_grad_weight_workspace(uint64_t n, uint32_t in, uint32_t out, int type);
 int opal_linear_grad_weight(opal_ctx *ctx, const void *d_dy, uint64_t lddy, const void *d_x, uint64_t ldx, int type, uint64_t n, uint32_t in,

@@ -5,8 +5,9 @@
 //   backward     h = dy g, xh = (x - m) r:  dx = r (h - mean(h) - xh mean(h xh));  dg = sum_rows dy xh,  db = sum_rows dy
 //   softmax      e_j = exp(s_j - max), Z = sum e_j:  loss = log Z + max - s_label, grad_j = scale (e_j / Z - [j is the label])
 //
-// A row of up to 2048 columns belongs to a wave, which holds it in registers (one read of memory, sums over the wave's lanes);
-// up to 8192 to a block of 256 threads in the same way; a longer one is read again by a block of 1024 for each pass.
+// A row belongs to a team of 16, 32 or 64 lanes (up to 128, 512, 2048 columns), which holds it in registers: one read of memory, sums
+// over the team's lanes; up to 8192 columns to a block of 256 threads in the same way; a longer one is read again by a block of
+// 1024 for each pass.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -17,16 +18,16 @@ namespace opal_head {
 
 constexpr int BLOCK = 256;
 
-// Sums and maxima over the TPR threads of a row: a wave, or the whole block (red: one float per wave and value, two buffers in
-// turn so that a block needs one barrier per reduction).
+// Sums and maxima over the TPR threads of a row: 16, 32 or 64 lanes, or the whole block (red: one float per wave and value, two
+// buffers in turn so that a block needs one barrier per reduction).
 template <int TPR> struct Team {
     float *red;
     int turn = 0;
     __device__ __forceinline__ float join(float v, bool take_max)
     {
-        v = take_max ? wave_max(v) : wave_sum(v);
-        if constexpr (TPR == WAVE) return v;
+        if constexpr (TPR <= WAVE) return take_max ? wave_max<TPR>(v) : wave_sum<TPR>(v);
         else {
+            v = take_max ? wave_max(v) : wave_sum(v);
             constexpr int NW = TPR / WAVE;
             float *r = red + (turn ^= NW);
             if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
@@ -40,11 +41,11 @@ template <int TPR> struct Team {
     __device__ __forceinline__ float max(float v) { return join(v, true); }
 };
 
-// A thread's share of a row: quads i * TPR + t, i < NQ = ceil(cols / (4 TPR)); all but the last are whole.
+// A thread's share of a row: quads i * TPR + t, i < NQ.  Teams within a wave have NQ = ceil(cols / (4 TPR)): all quads but the last are whole.
 template <int TPR, int NQ> __device__ __forceinline__ int quad_col(int i, int t) { return (i * TPR + t) * 4; }
-template <int NQ> __device__ __forceinline__ int quad_left(int i, int col, int cols)
+template <int TPR, int NQ> __device__ __forceinline__ int quad_left(int i, int col, int cols)
 {
-    return i < NQ - 1 ? 4 : cols - col;
+    return TPR <= WAVE && i < NQ - 1 ? 4 : cols - col;
 }
 
 template <class T> constexpr int type_of() { return __is_same(T, float) ? OPAL_F32 : __is_same(T, f16_t) ? OPAL_F16 : OPAL_BF16; }
@@ -55,7 +56,7 @@ __device__ __forceinline__ void load_row(const T *row, int t, int cols, float fi
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
         const int col = quad_col<TPR, NQ>(i, t);
-        v[i] = load4_typed(row, type_of<T>(), col, quad_left<NQ>(i, col, cols), fill);
+        v[i] = load4_typed(row, type_of<T>(), col, quad_left<TPR, NQ>(i, col, cols), fill);
     }
 }
 
@@ -72,42 +73,42 @@ __device__ __forceinline__ f32x4 param4(const float *p, int col, int left, float
     return p ? load4_typed(p, OPAL_F32, col, left, none) : f32x4{none, none, none, none};
 }
 
-template <class T, int TPR, int NQ> __global__ __launch_bounds__(BLOCK) void norm_kernel(const Norm g)
+template <class T, int TPR, int NQ, bool NT> __global__ __launch_bounds__(BLOCK) void norm_kernel(const Norm g)
 {
     __shared__ float red[2 * BLOCK / WAVE];
     Team<TPR> team{red};
     constexpr int RPB = BLOCK / TPR;
     const int t = threadIdx.x % TPR;
     const float cols = (float)g.cols;
-    for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < g.n; row += (uint64_t)gridDim.x * RPB) {
-        f32x4 x[NQ];
-        load_row<T, TPR, NQ>((const T *)g.x + row * g.ldx, t, g.cols, 0.f, x);
-        float s = 0.f;
+    const uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (row >= g.n) return;
+    f32x4 x[NQ];
+    load_row<T, TPR, NQ>((const T *)g.x + row * g.ldx, t, g.cols, 0.f, x);
+    float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NQ; i++) s += (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
-        const float mean = team.sum(s) / cols;      // a division: the mean of equal values is that value
-        s = 0.f;
+    for (int i = 0; i < NQ; i++) s += (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
+    const float mean = team.sum(s) / cols;      // a division: the mean of equal values is that value
+    s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NQ; i++)
+    for (int i = 0; i < NQ; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[i][e] -= mean;
-                if (quad_left<NQ>(i, quad_col<TPR, NQ>(i, t), g.cols) > e) s += x[i][e] * x[i][e];
-            }
-        const float rstd = 1.f / sqrtf(team.sum(s) / cols + g.eps);
-#pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            const int col = quad_col<TPR, NQ>(i, t), left = quad_left<NQ>(i, col, g.cols);
-            const f32x4 ga = param4(g.gamma, col, left, 1.f), be = param4(g.beta, col, left, 0.f);
-            f32x4 y;
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = x[i][e] * rstd * ga[e] + be[e];
-            store4_typed(g.y, g.y_type, row * g.ldy + col, left, y);
+        for (int e = 0; e < 4; e++) {
+            x[i][e] -= mean;
+            if (quad_left<TPR, NQ>(i, quad_col<TPR, NQ>(i, t), g.cols) > e) s += x[i][e] * x[i][e];
         }
-        if (t == 0) {
-            if (g.mean) g.mean[row] = mean;
-            if (g.rstd) g.rstd[row] = rstd;
-        }
+    const float rstd = 1.f / sqrtf(team.sum(s) / cols + g.eps);
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+        const int col = quad_col<TPR, NQ>(i, t), left = quad_left<TPR, NQ>(i, col, g.cols);
+        const f32x4 ga = param4(g.gamma, col, left, 1.f), be = param4(g.beta, col, left, 0.f);
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = x[i][e] * rstd * ga[e] + be[e];
+        store4_typed<NT>(g.y, g.y_type, row * g.ldy + col, left, y);
+    }
+    if (t == 0) {
+        if (g.mean) g.mean[row] = mean;
+        if (g.rstd) g.rstd[row] = rstd;
     }
 }
 
@@ -144,30 +145,57 @@ struct NormBack {
     uint64_t n; int cols;
     void *dx; int dx_type; uint64_t lddx;      // dx may be null
     float *part;                               // [blocks][2][cols]: dgamma, dbeta; null: not wanted
+    bool stream;                               // dx past the caches (stream_out)
 };
 
+// Threads of a block of the backward pass.  Short rows leave few bytes under way in a wave, so many waves share a block (and its one
+// partial sum); long ones fill a wave's registers.
+constexpr int back_threads(int TPR, int NQ) { return TPR > WAVE ? BLOCK : TPR * NQ <= 128 ? 1024 : TPR * NQ <= 256 ? 512 : BLOCK; }
+
 // Every thread keeps the sums of its own columns over the rows that its team visits; the teams of a block add theirs up in
-// order, and norm_sums_kernel adds the blocks': no atomics, the same bits every time.
-template <class TX, class TY, int TPR, int NQ> __global__ __launch_bounds__(BLOCK) void norm_back_kernel(const NormBack g)
+// order, and sum_parts_kernel adds the blocks': no atomics, the same bits every time.  The next row is asked for before the
+// present one is worked on.
+template <class TX, class TY, int TPR, int NQ> __global__ __launch_bounds__(back_threads(TPR, NQ)) void norm_back_kernel(const NormBack g)
 {
+    constexpr int THREADS = back_threads(TPR, NQ), RPB = THREADS / TPR, WAVES = THREADS / WAVE;
     __shared__ float red[2 * BLOCK / WAVE];
-    __shared__ f32x4 both[TPR == BLOCK ? 1 : 2 * NQ * TPR];
+    __shared__ f32x4 both[TPR <= WAVE ? 2 * NQ * TPR : 1];
     Team<TPR> team{red};
-    constexpr int RPB = BLOCK / TPR;
     const int t = threadIdx.x % TPR;
     const float cols = (float)g.cols;
+    const uint64_t step = (uint64_t)gridDim.x * RPB;
     f32x4 dg[NQ], db[NQ];
 #pragma unroll
     for (int i = 0; i < NQ; i++) dg[i] = db[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < g.n; row += (uint64_t)gridDim.x * RPB) {
+    uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    RawOf<TX> xr[NQ];
+    RawOf<TY> hr[NQ];
+    float mean_next = 0.f, rstd_next = 0.f;
+    auto ask = [&](uint64_t r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            const int col = quad_col<TPR, NQ>(i, t), left = quad_left<TPR, NQ>(i, col, g.cols);
+            xr[i] = load_raw_of((const TX *)g.x + r * g.ldx + col, left);
+            hr[i] = load_raw_of((const TY *)g.dy + r * g.lddy + col, left);
+        }
+        mean_next = g.mean[r];
+        rstd_next = g.rstd[r];
+    };
+    if (row < g.n) ask(row);
+    for (; row < g.n; row += step) {
         f32x4 x[NQ], h[NQ];
-        load_row<TX, TPR, NQ>((const TX *)g.x + row * g.ldx, t, g.cols, 0.f, x);
-        load_row<TY, TPR, NQ>((const TY *)g.dy + row * g.lddy, t, g.cols, 0.f, h);
-        const float mean = g.mean[row], rstd = g.rstd[row];
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            x[i] = decode_of(xr[i]);
+            h[i] = decode_of(hr[i]);
+        }
+        const float mean = mean_next, rstd = rstd_next;
+        // in place (dx over x or dy) other rows than this one are not touched: the next one may be read before this is written
+        if (row + step < g.n) ask(row + step);
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int i = 0; i < NQ; i++) {
-            const int col = quad_col<TPR, NQ>(i, t), left = quad_left<NQ>(i, col, g.cols);
+            const int col = quad_col<TPR, NQ>(i, t), left = quad_left<TPR, NQ>(i, col, g.cols);
             const f32x4 ga = param4(g.gamma, col, left, 1.f);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -184,17 +212,32 @@ template <class TX, class TY, int TPR, int NQ> __global__ __launch_bounds__(BLOC
         s1 = team.sum(s1) / cols;
 #pragma unroll
         for (int i = 0; i < NQ; i++) {
-            const int col = quad_col<TPR, NQ>(i, t), left = quad_left<NQ>(i, col, g.cols);
+            const int col = quad_col<TPR, NQ>(i, t), left = quad_left<TPR, NQ>(i, col, g.cols);
             f32x4 d;
 #pragma unroll
             for (int e = 0; e < 4; e++) d[e] = rstd * (h[i][e] - s0 - x[i][e] * s1);
-            store4_typed(g.dx, g.dx_type, row * g.lddx + col, left, d);
+            if (g.stream) store4_typed<true>(g.dx, g.dx_type, row * g.lddx + col, left, d);
+            else store4_typed<false>(g.dx, g.dx_type, row * g.lddx + col, left, d);
         }
     }
     if (!g.part) return;
-    if constexpr (TPR == WAVE) {
-        for (int w = 0; w < RPB; w++) {
-            if ((int)(threadIdx.x / TPR) == w) {
+    if constexpr (TPR <= WAVE) {
+#pragma unroll
+        for (int i = 0; i < NQ; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {                      // a wave's teams
+                if constexpr (TPR <= 16) {
+                    dg[i][e] = add_exchanged<16>(dg[i][e]);
+                    db[i][e] = add_exchanged<16>(db[i][e]);
+                }
+                if constexpr (TPR <= 32) {
+                    dg[i][e] = add_exchanged<32>(dg[i][e]);
+                    db[i][e] = add_exchanged<32>(db[i][e]);
+                }
+            }
+        const bool first = (threadIdx.x & 63) < TPR;           // a team of each wave
+        for (int w = 0; w < WAVES; w++) {
+            if ((int)(threadIdx.x / WAVE) == w && first) {
 #pragma unroll
                 for (int i = 0; i < NQ; i++) {
                     f32x4 *a = both + i * TPR + t, *b = both + (NQ + i) * TPR + t;
@@ -208,12 +251,12 @@ template <class TX, class TY, int TPR, int NQ> __global__ __launch_bounds__(BLOC
             }
             __syncthreads();
         }
-        if ((int)(threadIdx.x / TPR) != RPB - 1) return;      // the last team holds the block's sums
+        if ((int)(threadIdx.x / WAVE) != WAVES - 1 || !first) return;      // the last wave's team holds the block's sums
     }
     float *out = g.part + (uint64_t)blockIdx.x * 2 * g.cols;
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
-        const int col = quad_col<TPR, NQ>(i, t), left = quad_left<NQ>(i, col, g.cols);
+        const int col = quad_col<TPR, NQ>(i, t), left = quad_left<TPR, NQ>(i, col, g.cols);
         store4_typed(out, OPAL_F32, col, left, dg[i]);
         store4_typed(out, OPAL_F32, (uint64_t)g.cols + col, left, db[i]);
     }
@@ -260,20 +303,27 @@ template <class TX, class TY> __global__ __launch_bounds__(BLOCK) void norm_cols
     out[(uint64_t)g.cols + c] = db;
 }
 
-// out[c] = sum over parts of part[p * stride + c], c < width, in a fixed order; parts == 0 writes zeros.
-__global__ __launch_bounds__(1024) void sum_parts_kernel(const float *part, uint64_t parts, uint64_t stride, uint64_t width, float *out)
+// The sums over `parts` of [2][cols]: the first goes to out0, the second to out1 (either may be null), in a fixed order; parts == 0
+// writes zeros.  A block takes 16 columns with 64 groups of parts.
+__global__ __launch_bounds__(1024) void sum_parts_kernel(const float *part, uint32_t parts, uint32_t cols, float *out0, float *out1)
 {
-    __shared__ float acc[16][64];
-    const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const uint64_t col = (uint64_t)blockIdx.x * 64 + c;
+    __shared__ float acc[64][16];
+    const uint32_t c = threadIdx.x & 15, w = threadIdx.x >> 4;
+    const uint64_t col = (uint64_t)blockIdx.x * 16 + c, width = 2ull * cols;
     float s = 0.f;
-    if (col < width)
-        for (uint64_t p = w; p < parts; p += 16) s += part[p * stride + col];
+    if (col < width) {
+#pragma unroll 8
+        for (uint32_t p = w; p < parts; p += 64) s += part[p * width + col];
+    }
     acc[w][c] = s;
     __syncthreads();
+    for (uint32_t half = 32; half; half >>= 1) {
+        if (w < half) acc[w][c] += acc[w + half][c];
+        __syncthreads();
+    }
     if (w == 0 && col < width) {
-        for (int i = 1; i < 16; i++) s += acc[i][c];
-        out[col] = s;
+        float *out = col < cols ? out0 : out1;
+        if (out) out[col < cols ? col : col - cols] = acc[0][c];
     }
 }
 
@@ -307,56 +357,56 @@ __device__ __forceinline__ int softmax_label(const Softmax &g, uint64_t row, boo
     return bad ? -1 : l - 1;
 }
 
-template <class T, int TPR, int NQ> __global__ __launch_bounds__(BLOCK) void softmax_kernel(const Softmax g)
+template <class T, int TPR, int NQ, bool NT> __global__ __launch_bounds__(BLOCK) void softmax_kernel(const Softmax g)
 {
     __shared__ float red[2 * BLOCK / WAVE];
     Team<TPR> team{red};
     constexpr int RPB = BLOCK / TPR;
     const int t = threadIdx.x % TPR;
-    for (uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < g.n; row += (uint64_t)gridDim.x * RPB) {
-        const T *s = (const T *)g.s + row * g.lds;
-        f32x4 x[NQ];
-        load_row<T, TPR, NQ>(s, t, g.cols, -INFINITY, x);
-        bool bad = false;
-        const int label = softmax_label(g, row, bad);
-        const float at = label >= 0 && g.loss ? (float)s[label] : 0.f;  // here, before anybody writes: grad may be s
-        float top = -INFINITY;
+    const uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (row >= g.n) return;
+    const T *s = (const T *)g.s + row * g.lds;
+    f32x4 x[NQ];
+    load_row<T, TPR, NQ>(s, t, g.cols, -INFINITY, x);
+    bool bad = false;
+    const int label = softmax_label(g, row, bad);
+    const float at = label >= 0 && g.loss ? (float)s[label] : 0.f;  // here, before anybody writes: grad may be s
+    float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NQ; i++) top = fmaxf(top, fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3])));
-        top = team.max(top);
-        int best = 0;
-        if (g.out_class) {
-            int first = 0x7fffffff;                                    // the lowest class of the maximum
+    for (int i = 0; i < NQ; i++) top = fmaxf(top, fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3])));
+    top = team.max(top);
+    int best = 0;
+    if (g.out_class) {
+        int first = 0x7fffffff;                                    // the lowest class of the maximum
 #pragma unroll
-            for (int i = NQ - 1; i >= 0; i--)
+        for (int i = NQ - 1; i >= 0; i--)
 #pragma unroll
-                for (int e = 3; e >= 0; e--)
-                    if (x[i][e] == top) first = quad_col<TPR, NQ>(i, t) + e;
-            const float low = -team.max(first == 0x7fffffff ? -INFINITY : -(float)first);   // cols <= 2^20: exact in a float
-            best = low < (float)g.cols ? (int)low : 0;
+            for (int e = 3; e >= 0; e--)
+                if (x[i][e] == top) first = quad_col<TPR, NQ>(i, t) + e;
+        const float low = -team.max(first == 0x7fffffff ? -INFINITY : -(float)first);   // cols <= 2^20: exact in a float
+        best = low < (float)g.cols ? (int)low : 0;
+    }
+    const float shift = top == -INFINITY ? 0.f : top;
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < NQ; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[i][e] = expf(x[i][e] - shift);
+            z += x[i][e];
         }
-        const float shift = top == -INFINITY ? 0.f : top;
-        float z = 0.f;
+    z = team.sum(z);
+    if (t == 0) softmax_row(g, row, shift, z, best, label, bad, at);
+    if (g.grad) {
+        const float f = label < 0 || z == 0.f ? 0.f : g.scale / z;
+        const bool none = label < 0 || z == 0.f;
 #pragma unroll
-        for (int i = 0; i < NQ; i++)
+        for (int i = 0; i < NQ; i++) {
+            const int col = quad_col<TPR, NQ>(i, t);
+            f32x4 d;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[i][e] = expf(x[i][e] - shift);
-                z += x[i][e];
-            }
-        z = team.sum(z);
-        if (t == 0) softmax_row(g, row, shift, z, best, label, bad, at);
-        if (g.grad) {
-            const float f = label < 0 || z == 0.f ? 0.f : g.scale / z;
-            const bool none = label < 0 || z == 0.f;
-#pragma unroll
-            for (int i = 0; i < NQ; i++) {
-                const int col = quad_col<TPR, NQ>(i, t);
-                f32x4 d;
-#pragma unroll
-                for (int e = 0; e < 4; e++) d[e] = none ? 0.f : col + e == label ? x[i][e] * f - g.scale : x[i][e] * f;
-                store4_typed(g.grad, g.grad_type, row * g.ldg + col, quad_left<NQ>(i, col, g.cols), d);
-            }
+            for (int e = 0; e < 4; e++) d[e] = none ? 0.f : col + e == label ? x[i][e] * f - g.scale : x[i][e] * f;
+            store4_typed<NT>(g.grad, g.grad_type, row * g.ldg + col, quad_left<TPR, NQ>(i, col, g.cols), d);
         }
     }
 }
@@ -396,58 +446,74 @@ template <class T> __global__ __launch_bounds__(LONG) void softmax_long_kernel(c
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-constexpr int WAVE_COLS = 2048, BLOCK_COLS = 8192;
+constexpr int BLOCK_COLS = 8192;
 
-#define OPAL_NQ_CASES(LAUNCH, TPR, NQ) \
-    switch (NQ) {                      \
-    case 1: LAUNCH(TPR, 1); break;     \
-    case 2: LAUNCH(TPR, 2); break;     \
-    case 3: LAUNCH(TPR, 3); break;     \
-    case 4: LAUNCH(TPR, 4); break;     \
-    case 5: LAUNCH(TPR, 5); break;     \
-    case 6: LAUNCH(TPR, 6); break;     \
-    case 7: LAUNCH(TPR, 7); break;     \
-    default: LAUNCH(TPR, 8); break;    \
-    }
+// LAUNCH(TPR, NQ): the narrowest team whose rows fit, and its quads a thread
+#define OPAL_TEAMS(LAUNCH, cols)                                  \
+    if ((cols) <= 64) { LAUNCH(16, 1); }                          \
+    else if ((cols) <= 128) { LAUNCH(16, 2); }                    \
+    else if ((cols) <= 256) { LAUNCH(32, 2); }                    \
+    else if ((cols) <= 384) { LAUNCH(32, 3); }                    \
+    else if ((cols) <= 512) { LAUNCH(32, 4); }                    \
+    else if ((cols) <= 768) { LAUNCH(64, 3); }                    \
+    else if ((cols) <= 1024) { LAUNCH(64, 4); }                   \
+    else if ((cols) <= 1280) { LAUNCH(64, 5); }                   \
+    else if ((cols) <= 1536) { LAUNCH(64, 6); }                   \
+    else if ((cols) <= 1792) { LAUNCH(64, 7); }                   \
+    else if ((cols) <= 2048) { LAUNCH(64, 8); }                   \
+    else if ((cols) <= 4096) { LAUNCH(256, 4); }                  \
+    else if ((cols) <= 6144) { LAUNCH(256, 6); }                  \
+    else { LAUNCH(256, 8); }
 
 static unsigned row_grid(uint64_t n, int rows_per_block, int cus, int blocks_per_cu)
 {
     return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((n + rows_per_block - 1) / rows_per_block, (uint64_t)cus * blocks_per_cu));
 }
 
+static unsigned blocks_for(uint64_t n, int rows_per_block) { return (unsigned)((n + rows_per_block - 1) / rows_per_block); }
+
+// Results of more than the 256 MiB that the memory-side cache holds are written past it: 250 000 rows of 1564 in bf16, 423 -> 408 us.
+static bool stream_out(uint64_t n, uint64_t cols, int type) { return n * cols * type_bytes(type) > (256u << 20); }
+
 template <class T> static void run_norm(const Norm &g, int cus, hipStream_t st)
 {
-#define L(TPR, NQ) hipLaunchKernelGGL((norm_kernel<T, TPR, NQ>), dim3(row_grid(g.n, BLOCK / TPR, cus, 8)), dim3(BLOCK), 0, st, g)
-    if (g.cols <= WAVE_COLS) { OPAL_NQ_CASES(L, 64, (g.cols + 255) / 256) }
-    else if (g.cols <= BLOCK_COLS) { OPAL_NQ_CASES(L, 256, (g.cols + 1023) / 1024) }
+#define L(TPR, NQ)                                                                                                                  \
+    if (nt) hipLaunchKernelGGL((norm_kernel<T, TPR, NQ, true>), dim3(blocks_for(g.n, BLOCK / TPR)), dim3(BLOCK), 0, st, g);             \
+    else hipLaunchKernelGGL((norm_kernel<T, TPR, NQ, false>), dim3(blocks_for(g.n, BLOCK / TPR)), dim3(BLOCK), 0, st, g)
+    const bool nt = stream_out(g.n, g.cols, g.y_type);
+    if (g.cols <= BLOCK_COLS) { OPAL_TEAMS(L, g.cols) }
     else hipLaunchKernelGGL(norm_long_kernel<T>, dim3(row_grid(g.n, 1, cus, 2)), dim3(LONG), 0, st, g);
 #undef L
 }
 
 template <class T> static void run_softmax(const Softmax &g, int cus, hipStream_t st)
 {
-#define L(TPR, NQ) hipLaunchKernelGGL((softmax_kernel<T, TPR, NQ>), dim3(row_grid(g.n, BLOCK / TPR, cus, 8)), dim3(BLOCK), 0, st, g)
-    if (g.cols <= WAVE_COLS) { OPAL_NQ_CASES(L, 64, (g.cols + 255) / 256) }
-    else if (g.cols <= BLOCK_COLS) { OPAL_NQ_CASES(L, 256, (g.cols + 1023) / 1024) }
+#define L(TPR, NQ)                                                                                                                  \
+    if (nt) hipLaunchKernelGGL((softmax_kernel<T, TPR, NQ, true>), dim3(blocks_for(g.n, BLOCK / TPR)), dim3(BLOCK), 0, st, g);          \
+    else hipLaunchKernelGGL((softmax_kernel<T, TPR, NQ, false>), dim3(blocks_for(g.n, BLOCK / TPR)), dim3(BLOCK), 0, st, g)
+    const bool nt = g.grad && stream_out(g.n, g.cols, g.grad_type);
+    if (g.cols <= BLOCK_COLS) { OPAL_TEAMS(L, g.cols) }
     else hipLaunchKernelGGL(softmax_long_kernel<T>, dim3(row_grid(g.n, 1, cus, 2)), dim3(LONG), 0, st, g);
 #undef L
 }
 
-// Blocks of the backward pass, which is the number of partial sums: enough to fill the card, and none with less than eight rows
-// a team, below which the partial sums would be as much to read as the rows.
-constexpr uint64_t NORM_BACK_BLOCKS = 1024;
+// Blocks of the backward pass, which is the number of partial sums: enough waves to fill the card (two blocks a CU), and none with
+// less than four rows a team, below which the partial sums would be as much to read as the rows.
+constexpr uint64_t NORM_BACK_BLOCKS = 512;
 static uint64_t norm_back_blocks(uint64_t n, uint32_t cols)
 {
     if (cols > BLOCK_COLS) return std::min<uint64_t>((n + 63) / 64, 64);
-    const uint64_t rpb = cols <= WAVE_COLS ? BLOCK / WAVE : 1;
-    return std::min<uint64_t>((n + 8 * rpb - 1) / (8 * rpb), NORM_BACK_BLOCKS);
+#define ROWS(TPR, NQ) rows = back_threads(TPR, NQ) / TPR
+    uint64_t rows;
+    OPAL_TEAMS(ROWS, cols)
+#undef ROWS
+    return std::min<uint64_t>((n + 4 * rows - 1) / (4 * rows), cols <= 2048 ? NORM_BACK_BLOCKS : 2 * NORM_BACK_BLOCKS);
 }
 
 template <class TX, class TY> static void run_norm_back(const NormBack &g, unsigned blocks, int cus, hipStream_t st)
 {
-#define L(TPR, NQ) hipLaunchKernelGGL((norm_back_kernel<TX, TY, TPR, NQ>), dim3(blocks), dim3(BLOCK), 0, st, g)
-    if (g.cols <= WAVE_COLS) { OPAL_NQ_CASES(L, 64, (g.cols + 255) / 256) }
-    else if (g.cols <= BLOCK_COLS) { OPAL_NQ_CASES(L, 256, (g.cols + 1023) / 1024) }
+#define L(TPR, NQ) hipLaunchKernelGGL((norm_back_kernel<TX, TY, TPR, NQ>), dim3(blocks), dim3(back_threads(TPR, NQ)), 0, st, g)
+    if (g.cols <= BLOCK_COLS) { OPAL_TEAMS(L, g.cols) }
     else {
         if (g.part) hipLaunchKernelGGL((norm_cols_kernel<TX, TY>), dim3((g.cols + BLOCK - 1) / BLOCK, blocks), dim3(BLOCK), 0, st, g, (g.n + blocks - 1) / blocks);
         if (g.dx) hipLaunchKernelGGL((norm_back_long_kernel<TX, TY>), dim3(row_grid(g.n, 1, cus, 2)), dim3(LONG), 0, st, g);
@@ -460,11 +526,6 @@ template <class TX> static void run_norm_back_x(const NormBack &g, int dy_type, 
     if (dy_type == OPAL_F32) run_norm_back<TX, float>(g, blocks, cus, st);
     else if (dy_type == OPAL_F16) run_norm_back<TX, f16_t>(g, blocks, cus, st);
     else run_norm_back<TX, bf16_t>(g, blocks, cus, st);
-}
-
-static void sum_parts(const float *part, uint64_t parts, uint64_t stride, uint64_t width, float *out, hipStream_t st)
-{
-    hipLaunchKernelGGL(sum_parts_kernel, dim3((unsigned)((width + 63) / 64)), dim3(1024), 0, st, part, parts, stride, width, out);
 }
 
 // ------------------------------------------------------------------------------------------------ argument checks
@@ -543,15 +604,16 @@ extern "C" int opal_layer_norm_backward(opal_ctx *ctx, const void *d_dy, int dy_
     OPAL_HIP_CHECK(ctx, on.err);
     float *part = sums ? (float *)d_work : nullptr;
     if (n && (sums || d_dx)) {
-        const NormBack g{d_dy, lddy, d_x, ldx, d_gamma, d_mean, d_rstd, n, (int)cols, d_dx, dx_type, lddx, part};
+        const NormBack g{d_dy, lddy, d_x, ldx, d_gamma, d_mean, d_rstd, n, (int)cols, d_dx, dx_type, lddx, part, d_dx && stream_out(n, cols, dx_type)};
         if (x_type == OPAL_F32) run_norm_back_x<float>(g, dy_type, (unsigned)blocks, ctx->num_cus, ctx->stream);
         else if (x_type == OPAL_F16) run_norm_back_x<f16_t>(g, dy_type, (unsigned)blocks, ctx->num_cus, ctx->stream);
         else run_norm_back_x<bf16_t>(g, dy_type, (unsigned)blocks, ctx->num_cus, ctx->stream);
         OPAL_HIP_CHECK(ctx, hipGetLastError());
     }
-    if (d_dgamma) sum_parts(part, blocks, 2ull * cols, cols, d_dgamma, ctx->stream);
-    if (d_dbeta) sum_parts(part + cols, blocks, 2ull * cols, cols, d_dbeta, ctx->stream);
-    OPAL_HIP_CHECK(ctx, hipGetLastError());
+    if (sums) {
+        hipLaunchKernelGGL(sum_parts_kernel, dim3((2 * cols + 15) / 16), dim3(1024), 0, ctx->stream, part, (uint32_t)blocks, cols, d_dgamma, d_dbeta);
+        OPAL_HIP_CHECK(ctx, hipGetLastError());
+    }
     return OPAL_OK;
 }
 
@@ -603,12 +665,26 @@ constexpr int TILE[] = {64, 128, 256};
 
 static uint64_t tiles_of(uint64_t M, uint64_t N, int tile) { return ((M + TILE[tile] - 1) / TILE[tile]) * ((N + TILE[tile] - 1) / TILE[tile]); }
 
-// The largest tile that still gives every CU one (256 x 256: half of them, since its kernel is twice as fast): fewer bytes for the
-// same sums against idle CUs.
-static int pick_tile(uint64_t M, uint64_t N, int cus, bool big)
+// Larger tiles read fewer bytes for the same sums, smaller ones leave fewer CUs idle.
+//   128 x 128 from 1.5 tiles a CU on: 4096 x 512 x 1564 (416 tiles) 14.4 us against 15.1 with 64 x 64, 16384 x 1564 x 512 (512) 34.5 against
+//   49.3; below it 4096 x 1564 x 512 (128) 21.8 against 12.2, 32768 x 356 x 128 (256) 11.5 against 10.7.  32-bit types the same: 65536 x 356 x 100 (512) 58.1
+//   against 57.2, 16384 x 1564 x 512 (512) 201 against 213.
+//   256 x 256 (16-bit types, aligned) from one tile a CU on, four where the sums are short and its epilogue shows: 32768 x 1564 x 512 (256) 50.9
+//   us against 68.0 with 128 x 128, 65536 x 512 x 1564 (1792) 145 against 177; below it 16384 x 1564 x 512 (128) 36.6 against 34.5, 16384 x 512 x 1564
+//   (448) 59.0 against 49.6, 65536 x 356 x 128 (256) 19.3 against 17.6.
+static int pick_tile(uint64_t M, uint64_t N, uint64_t K, int cus, bool big)
 {
-    if (big && tiles_of(M, N, 2) * 2 >= (uint64_t)cus) return 2;
-    return tiles_of(M, N, 1) >= (uint64_t)cus ? 1 : 0;
+    if (big && tiles_of(M, N, 2) >= (uint64_t)cus * (K >= 1024 ? 1 : 4)) return 2;
+    return tiles_of(M, N, 1) * 2 >= (uint64_t)cus * 3 ? 1 : 0;
+}
+
+// The kernel for few rows, while its blocks (64 x 16 results, all of k) find a CU each: 64 x 1564 x 512 in 8.1 us against 10.3 with
+// 64 x 64 tiles, 512 rows (256 blocks) 8.3 against 10.5, 1024 rows 12.6 against 10.7; 2048 x 356 x 100 in 32 bits 7.1 against 11.4.  An
+// input gradient gathers W's columns there one by one: up to 16 rows (9.7 against 10.4 us; 64 rows 13.5 against 10.9).
+static bool few_rows(int product, uint64_t M, uint64_t N, int cus)
+{
+    if (product == GIN && M > 16) return false;
+    return ((M + 63) / 64) * ((N + 15) / 16) <= (uint64_t)cus;
 }
 
 static void set_tiles(Linear &g, int tile)
@@ -620,19 +696,47 @@ static void set_tiles(Linear &g, int tile)
 // 16-byte chunks straight into LDS need matrices and rows that begin on 16 bytes
 static bool aligned16(const void *p, uint64_t ld, int type) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * type_bytes(type) % 16 == 0; }
 
+static const char *past(const void *p, uint64_t rows, uint64_t ld, int type) { return p ? (const char *)p + rows * ld * type_bytes(type) : nullptr; }
+
 static int run_rows(opal_ctx *ctx, const char *who, Linear &g, int type, int product)
 {
     OnDevice on(ctx->device);
     OPAL_HIP_CHECK(ctx, on.err);
     const bool dma = aligned16(g.a, g.lda, type) && aligned16(g.b, g.ldb, type);
-    const int tile = pick_tile(g.M, g.N, ctx->num_cus, dma && type != OPAL_F32);
-    if (tiles_of(g.M, g.N, tile) >= (1ull << 31)) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": too many rows times columns for one call");
-    set_tiles(g, tile);
+    const int cus = ctx->num_cus;
+    int tile = few_rows(product, g.M, g.N, cus) ? 3 : pick_tile(g.M, g.N, g.K, cus, dma && type != OPAL_F32);
+    if (tile != 3 && tiles_of(g.M, g.N, tile) >= (1ull << 31)) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": too many rows times columns for one call");
     g.splits = 1;
     g.ksplit = g.K;
-    g.items = g.tm * g.tn;
-    g.blocks = std::min<uint32_t>(g.items, ctx->num_cus);
-    OPAL_HIP_CHECK(ctx, launch(g, type, product, tile, dma, ctx->stream));
+    auto run = [&](Linear &q, int t) {
+        if (t == 3) {
+            q.few = q.M <= 16 ? 1 : q.M <= 32 ? 2 : 4;
+            q.tm = (uint32_t)((q.M + 16 * q.few - 1) / (16 * q.few));
+            q.tn = (uint32_t)((q.N + 15) / 16);
+        } else set_tiles(q, t);
+        q.items = q.tm * q.tn;
+        q.blocks = std::min<uint32_t>(q.items, cus);
+        return launch(q, type, product, t, dma, ctx->stream);
+    };
+    // 256 x 256 tiles come in rounds of one a CU.  A last round of up to a quarter of the CUs goes to smaller tiles instead, in a
+    // launch of its own: 100 000 x 1564 x 512 (3.05 rounds) 239 -> 220 us; with two fifths, 60 001 x 512 x 1563 (6.43), 312 -> 328.
+    const uint64_t tn = (g.N + TILE[2] - 1) / TILE[2], tiles = tiles_of(g.M, g.N, 2), rounds = tiles / cus;
+    const uint64_t rows = rounds * cus / tn * TILE[2];
+    if (tile == 2 && rounds && rows < g.M && (tiles - rows / TILE[2] * tn) * 4 <= (uint64_t)cus) {
+        Linear q = g;
+        q.M = rows;
+        OPAL_HIP_CHECK(ctx, run(q, 2));
+        q = g;
+        q.M = g.M - rows;
+        q.a = past(g.a, rows, g.lda, type);
+        q.res = past(g.res, rows, g.ldr, g.res_type);
+        q.y = (void *)past(g.y, rows, g.ldy, g.y_type);
+        q.pre_in = past(g.pre_in, rows, g.ldp, type);
+        q.pre_out = (void *)past(g.pre_out, rows, g.ldp, type);
+        g = q;
+        tile = few_rows(product, g.M, g.N, cus) ? 3 : pick_tile(g.M, g.N, g.K, cus, false);
+    }
+    OPAL_HIP_CHECK(ctx, run(g, tile));
     return OPAL_OK;
 }
 
@@ -703,34 +807,44 @@ static Splits weight_splits(uint64_t n, uint32_t in, uint32_t out, int type)
     return {tile, (steps + per - 1) / per, per * step};
 }
 
-constexpr uint64_t COL_PARTS = 256;       // partial column sums of dy for the bias' gradient
-static uint64_t bias_parts(uint64_t n) { return std::min<uint64_t>((n + 31) / 32, COL_PARTS); }
-
 extern "C" uint64_t opal_linear_grad_weight_workspace(uint64_t n, uint32_t in, uint32_t out, int type)
 {
     if (!type_ok(type)) return 0;
     const Splits s = weight_splits(n, in, out, type);
-    return ((s.splits > 1 ? s.splits * in * out : 0) + bias_parts(n) * out) * sizeof(float);
+    return s.splits > 1 ? s.splits * ((uint64_t)in * out + out) * sizeof(float) : 0;
 }
 
 namespace opal_head {
-template <class T> __global__ __launch_bounds__(BLOCK) void col_sums_kernel(const T *x, uint64_t ld, uint64_t n, uint32_t cols, uint64_t rows, float *part)
+// The sum of the splits' matrices and of their row sums, in the splits' order: [splits][each] -> dw (rows of `cols`), [splits][out] -> db.
+// Reads what the product has just written; a thread adds up four neighbouring values, eight loads under way.
+__global__ __launch_bounds__(BLOCK) void sum_splits_kernel(const float *part, const float *rows, uint32_t splits, uint64_t each, uint32_t cols, uint32_t out,
+                                                           float *dw, uint64_t ld, float *db)
 {
-    const uint32_t c = blockIdx.x * BLOCK + threadIdx.x;
-    if (c >= cols) return;
-    const uint64_t beg = blockIdx.y * rows, end = beg + rows < n ? beg + rows : n;
-    float s = 0.f;
-    for (uint64_t r = beg; r < end; r++) s += (float)x[r * ld + c];
-    part[(uint64_t)blockIdx.y * cols + c] = s;
-}
-
-// out = the sum of the splits' matrices, in their order
-__global__ __launch_bounds__(BLOCK) void sum_splits_kernel(const float *part, uint64_t splits, uint64_t each, uint32_t cols, float *out, uint64_t ld)
-{
-    for (uint64_t i = (uint64_t)blockIdx.x * BLOCK + threadIdx.x; i < each; i += (uint64_t)gridDim.x * BLOCK) {
-        float s = part[i];
-        for (uint64_t p = 1; p < splits; p++) s += part[p * each + i];
-        out[i / cols * ld + i % cols] = s;
+    const uint64_t quads = dw ? (each + 3) / 4 : 0, all = quads + (db ? out : 0);
+    for (uint64_t i = (uint64_t)blockIdx.x * BLOCK + threadIdx.x; i < all; i += (uint64_t)gridDim.x * BLOCK) {
+        if (i >= quads) {
+            const uint64_t r = i - quads;
+            float s = rows[r];
+            for (uint32_t p = 1; p < splits; p++) s += rows[(uint64_t)p * out + r];
+            db[r] = s;
+            continue;
+        }
+        const int left = (int)std::min<uint64_t>(each - i * 4, 4);
+        f32x4 s;
+        if (left == 4) {
+            s = load4(part + i * 4);
+#pragma unroll 8
+            for (uint32_t p = 1; p < splits; p++) s += load4(part + p * each + i * 4);
+        } else {
+            s = load4_typed(part, OPAL_F32, i * 4, left);
+            for (uint32_t p = 1; p < splits; p++) s += load4_typed(part, OPAL_F32, p * each + i * 4, left);
+        }
+        if (ld == cols) store4_typed(dw, OPAL_F32, i * 4, left, s);
+        else
+            for (int e = 0; e < left; e++) {
+                const uint64_t at = i * 4 + e;
+                dw[at / cols * ld + at % cols] = s[e];
+            }
     }
 }
 }  // namespace opal_head
@@ -744,48 +858,34 @@ extern "C" int opal_linear_grad_weight(opal_ctx *ctx, const void *d_dy, uint64_t
     OPAL_TRY(check_shape(ctx, who, n, out, "out"));
     OPAL_TRY(check_matrix(ctx, who, "dy", d_dy, type, lddy, n, out));
     OPAL_TRY(check_matrix(ctx, who, "x", d_x, type, ldx, n, in));
-    OPAL_TRY(check_matrix(ctx, who, "dw", d_dw, OPAL_F32, lddw, out, in, true));
+    OPAL_TRY(check_matrix(ctx, who, "dw", d_dw, OPAL_F32, lddw, out, in));
     if (!type_ok(type)) return bad_arg(ctx, who, "unknown element type");
-    if (!d_dw && !d_dbias) return bad_arg(ctx, who, "neither dw nor dbias is asked for");
     const uint64_t need = opal_linear_grad_weight_workspace(n, in, out, type);
     if (need && (!d_work || work_bytes < need)) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": the workspace is smaller than opal_linear_grad_weight_workspace says");
     if (reinterpret_cast<uintptr_t>(d_work) % 16) return bad_arg(ctx, who, "the workspace must be 16-byte aligned");
     OnDevice on(ctx->device);
     OPAL_HIP_CHECK(ctx, on.err);
     const Splits s = weight_splits(n, in, out, type);
-    float *part = (float *)d_work;
     const uint64_t each = (uint64_t)in * out;
-    if (d_dw) {
-        Linear g{};
-        g.a = (const char *)d_dy; g.lda = lddy; g.b = (const char *)d_x; g.ldb = ldx;
-        g.M = out; g.N = in; g.K = n;
-        const bool dma = aligned16(d_dy, lddy, type) && aligned16(d_x, ldx, type);
-        const int tile = s.tile == 2 && !dma ? 1 : s.tile;
-        if (tiles_of(out, in, tile) * s.splits >= (1ull << 31)) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": in times out is too large for one call");
-        set_tiles(g, tile);
-        g.splits = (uint32_t)s.splits;
-        g.items = g.tm * g.tn * g.splits;
-        g.blocks = std::min<uint32_t>(g.items, ctx->num_cus);
-        g.ksplit = s.rows;
-        g.y = s.splits > 1 ? part : d_dw; g.y_type = OPAL_F32; g.ldy = s.splits > 1 ? in : lddw; g.y_split = each;
-        OPAL_HIP_CHECK(ctx, launch(g, type, GWT, tile, dma, ctx->stream));
-        if (s.splits > 1) {
-            hipLaunchKernelGGL(sum_splits_kernel, dim3((unsigned)std::min<uint64_t>((each + BLOCK - 1) / BLOCK, 4096)), dim3(BLOCK), 0, ctx->stream, part, s.splits, each, in, d_dw, lddw);
-            OPAL_HIP_CHECK(ctx, hipGetLastError());
-        }
-    }
-    if (d_dbias) {
-        float *bp = part + (s.splits > 1 ? s.splits * each : 0);
-        const uint64_t parts = bias_parts(n);
-        if (n) {
-            const uint64_t rows = (n + parts - 1) / parts;
-            const dim3 grid((out + BLOCK - 1) / BLOCK, (unsigned)parts);
-            if (type == OPAL_F32) hipLaunchKernelGGL(col_sums_kernel<float>, grid, dim3(BLOCK), 0, ctx->stream, (const float *)d_dy, lddy, n, out, rows, bp);
-            else if (type == OPAL_F16) hipLaunchKernelGGL(col_sums_kernel<f16_t>, grid, dim3(BLOCK), 0, ctx->stream, (const f16_t *)d_dy, lddy, n, out, rows, bp);
-            else hipLaunchKernelGGL(col_sums_kernel<bf16_t>, grid, dim3(BLOCK), 0, ctx->stream, (const bf16_t *)d_dy, lddy, n, out, rows, bp);
-            OPAL_HIP_CHECK(ctx, hipGetLastError());
-        }
-        sum_parts(bp, parts, out, out, d_dbias, ctx->stream);
+    float *part = s.splits > 1 ? (float *)d_work : nullptr, *rows = part ? part + s.splits * each : nullptr;
+    const bool dma = aligned16(d_dy, lddy, type) && aligned16(d_x, ldx, type);
+    const int tile = s.tile == 2 && !dma ? 1 : s.tile;
+    Linear g{};
+    g.a = (const char *)d_dy; g.lda = lddy; g.b = (const char *)d_x; g.ldb = ldx;
+    g.M = out; g.N = in; g.K = n;
+    if (tiles_of(g.M, g.N, tile) * s.splits >= (1ull << 31)) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": in times out is too large for one call");
+    set_tiles(g, tile);
+    g.splits = (uint32_t)s.splits;
+    g.ksplit = s.rows;
+    g.items = g.tm * g.tn * g.splits;
+    g.blocks = std::min<uint32_t>(g.items, ctx->num_cus);
+    g.y = part ? part : d_dw; g.y_type = OPAL_F32; g.ldy = part ? in : lddw; g.y_split = each;
+    g.colsum = d_dbias ? (part ? rows : d_dbias) : nullptr;
+    OPAL_HIP_CHECK(ctx, launch(g, type, GWT, tile, dma, ctx->stream));
+    if (part) {
+        const uint64_t work = (each + 3) / 4 + out;
+        hipLaunchKernelGGL(sum_splits_kernel, dim3((unsigned)std::min<uint64_t>((work + BLOCK - 1) / BLOCK, 8192)), dim3(BLOCK), 0, ctx->stream, part, rows,
+                           (uint32_t)s.splits, each, in, out, d_dw, lddw, d_dbias);
         OPAL_HIP_CHECK(ctx, hipGetLastError());
     }
     return OPAL_OK;

@@ -29,6 +29,8 @@ struct Linear {
     uint64_t y_split;             // elements between two splits' outputs
     const void *pre_in; void *pre_out; uint64_t ldp;   // the element type of the product
     int act;
+    float *colsum;                // GWT: sums of dy's rows, [splits][M], by the tiles at n = 0; or null
+    uint32_t few;                 // rows of a block of the kernel for few rows, in sixteens
     uint32_t items, blocks;       // tiles times splits, and the blocks that share them (opal_linear_big.h)
 };
 
@@ -247,6 +249,14 @@ template <class T, int R, bool KC, int NT, bool DMA> struct Operand {
     }
 };
 
+// the eight values of a fragment's lane, added up in 32 bits
+template <class T> __device__ __forceinline__ float sum8(s16x8 f)
+{
+    struct V { T v[8]; };
+    const V x = __builtin_bit_cast(V, f);
+    return (((float)x.v[0] + (float)x.v[1]) + ((float)x.v[2] + (float)x.v[3])) + (((float)x.v[4] + (float)x.v[5]) + ((float)x.v[6] + (float)x.v[7]));
+}
+
 template <class T> __device__ __forceinline__ f32x16 mfma16(s16x8 a, s16x8 b, f32x16 c)
 {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -263,6 +273,28 @@ __device__ __forceinline__ uint32_t xcd_tile(uint32_t b, uint32_t total)
 {
     const uint32_t x = b & 7u, per = total >> 3, extra = total & 7u;
     return x * per + (x < extra ? x : extra) + (b >> 3);
+}
+
+// The epilogue of four neighbouring results of a row, `ncol` of them the matrix's
+template <class T, int P> __device__ __forceinline__ void finish_quad(const Linear &g, f32x4 v, uint64_t m, uint64_t n, int ncol, f32x4 bias, uint64_t split)
+{
+    constexpr int own = __is_same(T, float) ? OPAL_F32 : __is_same(T, f16_t) ? OPAL_F16 : OPAL_BF16;
+    if constexpr (P == FWD) {
+        v += bias;
+        if (g.pre_out) store4_typed(g.pre_out, own, m * g.ldp + n, ncol, v);
+        if (g.act)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = act_value(v[e], g.act);
+    }
+    if constexpr (P == GIN) {
+        if (g.act) {
+            const f32x4 z = load4_typed(g.pre_in, own, m * g.ldp + n, ncol);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] *= act_slope(z[e], g.act);
+        }
+    }
+    if (P != GWT && g.res) v += load4_typed(g.res, g.res_type, m * g.ldr + n, ncol);
+    store4_typed(g.y, g.y_type, split * g.y_split + m * g.ldy + n, ncol, v);
 }
 
 template <class T, int P, int BM, int BN, int WM, int WN, bool DMA>
@@ -300,6 +332,10 @@ __global__ __launch_bounds__(WM * WN * WAVE) void linear_kernel(const Linear g)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
 
+    const bool sum_rows = P == GWT && n0 == 0 && wave % WN == 0 && g.colsum;      // one wave for each block of rows
+    float colsum[TM];
+#pragma unroll
+    for (int i = 0; i < TM; i++) colsum[i] = 0.f;
     uint64_t krem = kend - kbeg;
     char *cur = lds, *nxt = lds + STAGE;
     if (krem) {
@@ -328,6 +364,12 @@ __global__ __launch_bounds__(WM * WN * WAVE) void linear_kernel(const Linear g)
             for (int i = 0; i < TM; i++) OA::frag16(la, wm + i * 32, fa[i]);
 #pragma unroll
             for (int j = 0; j < TN; j++) OB::frag16(lb, wn + j * 32, fb[j]);
+            if (P == GWT && sum_rows) {
+#pragma unroll
+                for (int i = 0; i < TM; i++)
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) colsum[i] += sum8<T>(fa[i][kk]);
+            }
 #pragma unroll
             for (int kk = 0; kk < 4; kk++)
 #pragma unroll
@@ -342,6 +384,9 @@ __global__ __launch_bounds__(WM * WN * WAVE) void linear_kernel(const Linear g)
                 for (int i = 0; i < TM; i++) fa[i] = OA::frag32(la, wm + i * 32, kk);
 #pragma unroll
                 for (int j = 0; j < TN; j++) fb[j] = OB::frag32(lb, wn + j * 32, kk);
+                if (P == GWT && sum_rows)
+#pragma unroll
+                    for (int i = 0; i < TM; i++) colsum[i] += (fa[i][0] + fa[i][1]) + (fa[i][2] + fa[i][3]);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
 #pragma unroll
@@ -362,6 +407,15 @@ __global__ __launch_bounds__(WM * WN * WAVE) void linear_kernel(const Linear g)
         cur = nxt;
         nxt = s;
         krem = more ? krem - STEP : 0;
+    }
+
+    if (P == GWT && sum_rows) {
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            const float s = colsum[i] + __shfl_xor(colsum[i], 32, WAVE);      // lanes l and l + 32 held the row's halves of k
+            const uint64_t m = m0 + wm + i * 32 + (lane & 31);
+            if (lane < 32 && m < g.M) g.colsum[split * g.M + m] = s;
+        }
     }
 
     // Epilogue: each wave turns 32 rows at a time in its own part of the LDS, so that neighbouring lanes hold neighbouring
@@ -388,32 +442,105 @@ __global__ __launch_bounds__(WM * WN * WAVE) void linear_kernel(const Linear g)
             const uint64_t m = m0 + wm + i * 32 + r;
             f32x4 v = *reinterpret_cast<const f32x4 *>(turn + r * EP_LD + col);
             if (m >= g.M || !ncol) continue;
-            if constexpr (P == FWD) {
-                v += bias;
-                if (g.pre_out) store4_typed(g.pre_out, __is_same(T, float) ? OPAL_F32 : __is_same(T, f16_t) ? OPAL_F16 : OPAL_BF16, m * g.ldp + n, ncol, v);
-                if (g.act)
-                    for (int e = 0; e < 4; e++) v[e] = act_value(v[e], g.act);
-            }
-            if constexpr (P == GIN) {
-                if (g.act) {
-                    const f32x4 z = load4_typed(g.pre_in, __is_same(T, float) ? OPAL_F32 : __is_same(T, f16_t) ? OPAL_F16 : OPAL_BF16, m * g.ldp + n, ncol);
-                    for (int e = 0; e < 4; e++) v[e] *= act_slope(z[e], g.act);
-                }
-            }
-            if (P != GWT && g.res) v += load4_typed(g.res, g.res_type, m * g.ldr + n, ncol);
-            store4_typed(g.y, g.y_type, split * g.y_split + m * g.ldy + n, ncol, v);
+            finish_quad<T, P>(g, v, m, n, ncol, bias, split);
         }
         wave_order();
     }
 }
 
+// ------------------------------------------------------------------------------------------------ few rows
+// FWD and GIN with few rows: reading W once is all there is to do, and what counts is that all of the card asks for it at once.  A
+// block takes 16 columns and 16 TM rows; its eight waves share the k between them, 32 (16 for 32-bit types) at a time, operands straight from
+// memory to v_mfma_f32_16x16x32 / 16x16x4_f32, and add up in LDS.  No LDS on the way in, no barrier but one.
+constexpr int FEW_WAVES = 8;
+
+// A fragment's lane: EPC values of k from k0 on of line r (KC), or column r of lines k0 .. (MC); beyond the matrix: zeros
+template <class T, bool KC> __device__ __forceinline__ u32x4 lane_k(const T *p, uint64_t ld, uint64_t r, bool in, uint64_t k0, uint64_t K)
+{
+    constexpr int EPC = 16 / sizeof(T);
+    u32x4 v = {0, 0, 0, 0};
+    if (!in || k0 >= K) return v;
+    const int left = K - k0 < (uint64_t)EPC ? (int)(K - k0) : EPC;
+    if (KC && left == EPC) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Any { uint32_t w[4]; };
+        const Any a = *reinterpret_cast<const Any *>(p + r * ld + k0);
+        return u32x4{a.w[0], a.w[1], a.w[2], a.w[3]};
+    }
+#pragma unroll
+    for (int e = 0; e < EPC; e++)
+        if (e < left) {
+            const T *q = KC ? p + r * ld + k0 + e : p + (k0 + e) * ld + r;
+            if constexpr (sizeof(T) == 4) v[e] = *reinterpret_cast<const uint32_t *>(q);
+            else v[e / 2] |= (uint32_t)*reinterpret_cast<const uint16_t *>(q) << (16 * (e & 1));
+        }
+    return v;
+}
+
+template <class T> __device__ __forceinline__ f32x4 mfma_few(u32x4 a, u32x4 b, f32x4 c)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    if constexpr (__is_same(T, bf16_t)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else if constexpr (__is_same(T, f16_t)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+        return c;
+    }
+#else
+    return c;
+#endif
+}
+
+template <class T, int P, int TM> __global__ __launch_bounds__(FEW_WAVES * WAVE) void linear_few_kernel(const Linear g)
+{
+    constexpr int EPC = 16 / sizeof(T), STEP = 4 * EPC, U = TM == 1 ? 8 : 4;
+    __shared__ f32x4 red[FEW_WAVES][TM][WAVE];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, kq = (lane >> 4) * EPC;
+    const uint64_t n0 = (uint64_t)(blockIdx.x % g.tn) * 16, m0 = (uint64_t)(blockIdx.x / g.tn) * (16 * TM);
+    const T *A = (const T *)g.a, *B = (const T *)g.b;
+    f32x4 acc[TM];
+#pragma unroll
+    for (int i = 0; i < TM; i++) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (uint64_t k = (uint64_t)wave * STEP; k < g.K; k += (uint64_t)U * FEW_WAVES * STEP) {
+        u32x4 b[U], a[U][TM];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint64_t ku = k + (uint64_t)u * FEW_WAVES * STEP + kq;
+            b[u] = lane_k<T, P == FWD>(B, g.ldb, n0 + r16, n0 + r16 < g.N, ku, g.K);
+#pragma unroll
+            for (int i = 0; i < TM; i++) a[u][i] = lane_k<T, true>(A, g.lda, m0 + i * 16 + r16, m0 + i * 16 + r16 < g.M, ku, g.K);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < TM; i++) acc[i] = mfma_few<T>(b[u], a[u][i], acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < TM; i++) red[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (threadIdx.x >= TM * WAVE) return;
+    f32x4 v = red[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < FEW_WAVES; w++) v += red[w][wave][lane];
+    const uint64_t m = m0 + wave * 16 + r16, n = n0 + (lane >> 4) * 4;           // four columns of a row
+    if (m >= g.M || n >= g.N) return;
+    const int ncol = g.N - n < 4 ? (int)(g.N - n) : 4;
+    finish_quad<T, P>(g, v, m, n, ncol, P == FWD && g.bias ? load4_typed(g.bias, OPAL_F32, n, ncol) : f32x4{0.f, 0.f, 0.f, 0.f}, 0);
+}
+
 // The launch of one product in one element type (opal_linear_{f32,f16,bf16}.hip); tile: 0 = 64 x 64, 1 = 128 x 128, 2 = 256 x 256
-// (16-bit types on the aligned path only).
+// (16-bit types on the aligned path only), 3 = few rows (g.few x 16).
 template <class T> hipError_t launch_linear(const Linear &g, int product, int tile, bool dma, hipStream_t stream);
 
 #define OPAL_LINEAR_CASE(T, P, TILE, BM, BN, WM, WN, D)                                                                              \
     if (product == P && tile == TILE && dma == D) {                                                                                  \
         hipLaunchKernelGGL((linear_kernel<T, P, BM, BN, WM, WN, D>), dim3(g.tm * g.tn * g.splits), dim3(WM * WN * WAVE), 0, stream, g); \
+        return hipGetLastError();                                                                                                    \
+    }
+#define OPAL_LINEAR_FEW(T, P, TM)                                                                                                   \
+    if (product == P && tile == 3 && g.few == TM) {                                                                                  \
+        hipLaunchKernelGGL((linear_few_kernel<T, P, TM>), dim3(g.tm * g.tn), dim3(FEW_WAVES * WAVE), 0, stream, g);                   \
         return hipGetLastError();                                                                                                    \
     }
 #define OPAL_LINEAR_CASES(T, P)                       \

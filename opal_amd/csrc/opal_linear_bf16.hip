@@ -8,6 +8,12 @@ template <> hipError_t launch_linear<bf16_t>(const Linear &g, int product, int t
     OPAL_LINEAR_CASES(bf16_t, FWD)
     OPAL_LINEAR_CASES(bf16_t, GIN)
     OPAL_LINEAR_CASES(bf16_t, GWT)
+    OPAL_LINEAR_FEW(bf16_t, FWD, 1)
+    OPAL_LINEAR_FEW(bf16_t, FWD, 2)
+    OPAL_LINEAR_FEW(bf16_t, FWD, 4)
+    OPAL_LINEAR_FEW(bf16_t, GIN, 1)
+    OPAL_LINEAR_FEW(bf16_t, GIN, 2)
+    OPAL_LINEAR_FEW(bf16_t, GIN, 4)
     return hipErrorInvalidValue;
 }
 }  // namespace opal_head

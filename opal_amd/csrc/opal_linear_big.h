@@ -70,8 +70,8 @@ template <int P, bool IS_A> struct Ring {
     {
         return ((uint32_t)((KC ? rows : kval) - 1) * ld + (uint32_t)(KC ? kval : rows) * 2u + 15u) & ~15u;
     }
-    // Fragments of COUNT times 32 rows from r0 on and of the 32 k that begin at 16 kk: k = 8 (lane / 32) + 0..7 of 16.
-    template <int COUNT> __device__ __forceinline__ static void frags(const char *lds, int r0, int kk, s16x8 (&f)[2][COUNT])
+    // Fragments of COUNT times 32 rows from r0 on, the block `rot` first, and of the 32 k that begin at 16 kk: k = 8 (lane / 32) + 0..7 of 16.
+    template <int COUNT> __device__ __forceinline__ static void frags(const char *lds, int r0, int rot, int kk, s16x8 (&f)[2][COUNT])
     {
         const int lane = threadIdx.x & 63;
         if constexpr (KC) {
@@ -86,7 +86,8 @@ template <int P, bool IS_A> struct Ring {
 #pragma unroll
             for (int i = 0; i < COUNT; i += 2) {
                 uint64_t x[8];
-                read_tr8<4 * BIG * 2, 16 * BIG * 2>(lds_place(lds) + tr_place<BIG>(r0 + i * 32), lds_place(lds) + tr_place<BIG>(r0 + i * 32 + 32), x);
+                read_tr8<4 * BIG * 2, 16 * BIG * 2>(lds_place(lds) + tr_place<BIG>(r0 + ((i + rot) & (COUNT - 1)) * 32),
+                                                     lds_place(lds) + tr_place<BIG>(r0 + ((i + 1 + rot) & (COUNT - 1)) * 32), x);
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     f[s][i] = join_tr(x[2 * s], x[2 * s + 1]);
@@ -243,7 +244,7 @@ __device__ __forceinline__ void store1(void *base, int type, uint64_t at, float 
     else ((bf16_t *)base)[at] = (bf16_t)v;
 }
 template <class T, int P, int ACT>
-__device__ __forceinline__ void epilogue_any(const Linear &g, const BigItem &c, const f32x16 (&acc)[4][2], float *turn, int wm, int wn)
+__device__ __forceinline__ void epilogue_any(const Linear &g, const BigItem &c, const f32x16 (&acc)[4][2], float *turn, int wm, int wn, int rot)
 {
     constexpr int own = own_type<T>();
     const int lane = threadIdx.x & 63;
@@ -267,7 +268,7 @@ __device__ __forceinline__ void epilogue_any(const Linear &g, const BigItem &c, 
         wave_order();
 #pragma unroll 2
         for (int row = 0; row < 8; row++) {                    // a lane a column
-            const uint64_t m = m0 + s * 8 + row;
+            const uint64_t m = m0 + (((s >> 2) + rot) & 3) * 32 + (s & 3) * 8 + row;
             float v = turn[row * 64 + (((lane >> 2) ^ (row * 2)) * 4) + (lane & 3)];
             if (m < g.M && n < g.N) {
                 if (P == GIN && ACT) v *= act_slope(load1(g.pre_in, own, m * g.ldp + n), ACT);
@@ -315,7 +316,7 @@ template <class T> __device__ __forceinline__ void store_joined(void *to, uint64
 }
 
 template <class T, int P, int ACT, bool Y32, bool RES>
-__device__ __forceinline__ void epilogue_plain(const Linear &g, const BigItem &c, const f32x16 (&acc)[4][2], int wm, int wn)
+__device__ __forceinline__ void epilogue_plain(const Linear &g, const BigItem &c, const f32x16 (&acc)[4][2], int wm, int wn, int rot)
 {
     constexpr int own = own_type<T>();
     const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -324,7 +325,7 @@ __device__ __forceinline__ void epilogue_plain(const Linear &g, const BigItem &c
     constexpr bool with_res = RES, with_pre = P == GIN && ACT;      // known here: a load that might not be used would be waited for in the loop
     RawQuad res[2][4], pre[2][4];
     auto ask = [&](int t) __attribute__((always_inline)) {
-        const uint32_t m = m0 + (t >> 1) * 32;
+        const uint32_t m = m0 + (((t >> 1) + rot) & 3) * 32;
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const uint32_t n = nq + (t & 1) * 32 + q * 8;
@@ -343,7 +344,7 @@ __device__ __forceinline__ void epilogue_plain(const Linear &g, const BigItem &c
                 if (nq + j * 32 + q * 8 < N) bias[j][q] = load4(g.bias + nq + j * 32 + q * 8);
 #pragma unroll
     for (int t = 0; t < 8; t++) {
-        const uint32_t m = m0 + (t >> 1) * 32;
+        const uint32_t m = m0 + (((t >> 1) + rot) & 3) * 32;
         f32x16 v = acc[t >> 1][t & 1];
         if ((with_res || with_pre) && t < 7) ask(t + 1);
         if (P == FWD) {
@@ -400,15 +401,19 @@ __device__ __forceinline__ void epilogue_plain(const Linear &g, const BigItem &c
 // chunk.  sub: the step's 32 k within A's stage.  fresh: the next step begins a new stage of A; last: of the tile.
 template <class T, int P, bool CUT>
 __device__ __forceinline__ void big_step(Feed<P> &feed, f32x16 (&acc)[4][2], char *lds, uint32_t slot_a, uint32_t slot_b, int sub, bool fresh, bool last, int wave,
-                                         int half, int &landed, int ctail)
+                                         int half, int &landed, int ctail, bool sum_rows, float &colsum)
 {
     using RA = Ring<P, true>;
     using RB = Ring<P, false>;
     const char *sa = lds + slot_a * RA::BYTES, *sb = lds + RA::N * RA::BYTES + slot_b * RB::BYTES;
     const int wm = half * 128, wn = (wave & 3) * 64;
     s16x8 fa[2][4], fb[2][2];
-    RA::template frags<4>(sa, wm, sub * 2, fa);
-    RB::template frags<2>(sb, wn, 0, fb);
+    RA::template frags<4>(sa, wm, P == GWT ? wave & 3 : 0, sub * 2, fa);
+    RB::template frags<2>(sb, wn, 0, 0, fb);
+    if (P == GWT && sum_rows) {                // of dy: this wave's first block, which its rotation makes another than its neighbours'
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) colsum += sum8<T>(fa[kk][0]);
+    }
     if constexpr (CUT) {
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
@@ -489,7 +494,10 @@ template <class T, int P, int ACT, bool Y32, bool RES> __global__ __launch_bound
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
-        const uint64_t count = big_item<P>(reload(), ci).count;
+        const BigItem now = big_item<P>(reload(), ci);
+        const uint64_t count = now.count;
+        const bool sum_rows = P == GWT && now.n0 == 0 && reload().colsum;
+        float colsum = 0.f;
         const uint32_t steps = (uint32_t)((count + BIG_STEP - 1) / BIG_STEP);
         const int tail = (int)(count - (uint64_t)(steps - 1) * BIG_STEP);
         const bool odd = P != GWT && (tail & 7);
@@ -498,13 +506,13 @@ template <class T, int P, int ACT, bool Y32, bool RES> __global__ __launch_bound
 #pragma unroll 1
         for (uint32_t s = 0; s < whole; s++) {
             const bool fresh = sub == RA::PARTS - 1 || s + 1 == steps;
-            big_step<T, P, false>(feed, acc, lds, slot_a, slot_b, sub, fresh, s + 1 == steps, wave, half, landed, 0);
+            big_step<T, P, false>(feed, acc, lds, slot_a, slot_b, sub, fresh, s + 1 == steps, wave, half, landed, 0, sum_rows, colsum);
             slot_b = slot_b + 1 == RB::N ? 0 : slot_b + 1;
             if (fresh) slot_a = slot_a + 1 == RA::N ? 0 : slot_a + 1;
             sub = fresh ? 0 : sub + 1;
         }
         if (odd) {
-            big_step<T, P, true>(feed, acc, lds, slot_a, slot_b, sub, true, true, wave, half, landed, tail);
+            big_step<T, P, true>(feed, acc, lds, slot_a, slot_b, sub, true, true, wave, half, landed, tail, false, colsum);
             slot_b = slot_b + 1 == RB::N ? 0 : slot_b + 1;
             slot_a = slot_a + 1 == RA::N ? 0 : slot_a + 1;
         }
@@ -514,9 +522,15 @@ template <class T, int P, int ACT, bool Y32, bool RES> __global__ __launch_bound
         const Linear &g = reload();
         const BigItem c = big_item<P>(g, ci);
         constexpr int own = own_type<T>();
+        if (P == GWT && sum_rows) {
+            colsum += __shfl_xor(colsum, 32, WAVE);            // the two halves of each 16 k
+            const uint32_t m = c.m0 + half * 128 + (wave & 3) * 32 + (threadIdx.x & 31);
+            if ((threadIdx.x & 32) == 0 && m < g.M) g.colsum[c.split * g.M + m] = colsum;
+        }
         const bool plain = (g.N - c.n0 >= BIG || g.N % 8 == 0) && g.y_type == (Y32 ? OPAL_F32 : own) && (!RES || g.res_type == OPAL_F32 || g.res_type == own);
-        if (plain) epilogue_plain<T, P, ACT, Y32, RES>(g, c, acc, half * 128, (wave & 3) * 64);
-        else epilogue_any<T, P, ACT>(g, c, acc, reinterpret_cast<float *>(lds + RA::N * RA::BYTES + RB::N * RB::BYTES + wave * BIG_TURN), half * 128, (wave & 3) * 64);
+        if (plain) epilogue_plain<T, P, ACT, Y32, RES>(g, c, acc, half * 128, (wave & 3) * 64, P == GWT ? wave & 3 : 0);
+        else epilogue_any<T, P, ACT>(g, c, acc, reinterpret_cast<float *>(lds + RA::N * RA::BYTES + RB::N * RB::BYTES + wave * BIG_TURN), half * 128, (wave & 3) * 64,
+                                         P == GWT ? wave & 3 : 0);
         ci += g.blocks;
         if (ci >= g.items) break;
         if (half) asm volatile("s_barrier" ::: "memory");

@@ -7,6 +7,12 @@ template <> hipError_t launch_linear<float>(const Linear &g, int product, int ti
     OPAL_LINEAR_CASES(float, FWD)
     OPAL_LINEAR_CASES(float, GIN)
     OPAL_LINEAR_CASES(float, GWT)
+    OPAL_LINEAR_FEW(float, FWD, 1)
+    OPAL_LINEAR_FEW(float, FWD, 2)
+    OPAL_LINEAR_FEW(float, FWD, 4)
+    OPAL_LINEAR_FEW(float, GIN, 1)
+    OPAL_LINEAR_FEW(float, GIN, 2)
+    OPAL_LINEAR_FEW(float, GIN, 4)
     return hipErrorInvalidValue;
 }
 }  // namespace opal_head

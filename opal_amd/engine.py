@@ -211,6 +211,9 @@ class Engine:
         torch.cuda.set_device(self.device)
         stream = torch.cuda.current_stream(self.device).cuda_stream if use_torch_stream else None
         self._stream = stream or 0
+        self._lib = lib()
+        # the handle of a device's current stream: the short way where torch has it (0.1 us against 1.9)
+        self._current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
         self._types = {torch.float32: _lib.OPAL_F32, torch.float16: _lib.OPAL_F16, torch.bfloat16: _lib.OPAL_BF16}
         h = C.c_void_p()
         check(lib().opal_ctx_create(device, stream, C.byref(h)))
@@ -374,39 +377,60 @@ class Engine:
     # Matrices are torch tensors [n, cols] on the engine's GPU, float32 / float16 / bfloat16, whose last stride is 1 and whose row
     # stride is at least cols (a view into wider rows is fine); new ones get rows of a multiple of 16 bytes.  The work runs on the
     # engine's stream; when torch's current stream is another one, the two are ordered before and after the call.
-    def _matrix(self, x, name, shape=None, dtype=None):
-        if not isinstance(x, self.torch.Tensor) or x.device != self.device or x.dim() != 2:
-            raise ValueError("%s must be a matrix (2-d tensor) on %s" % (name, self.device))
-        if x.dtype not in self._types or (dtype is not None and x.dtype != dtype):
-            raise ValueError("%s is %s: must be %s" % (name, x.dtype, dtype or "float32, float16 or bfloat16"))
-        if shape is not None and tuple(x.shape) != shape:
-            raise ValueError("%s is %s: must be %s" % (name, tuple(x.shape), shape))
-        n, cols = x.shape
-        ld = x.stride(0) if n > 1 else cols
-        if cols < 1 or (cols > 1 and x.stride(1) != 1) or ld < cols:
+    # (What every call does is kept short: a call for one read is as long as its host side.)
+    def _matrix(self, x, name, rows=None, cols=None, dtype=None):
+        """(address, element type, row stride, rows, columns) of a matrix argument, checked."""
+        try:
+            n, c = x.shape
+            ld, one = x.stride()
+            kind = self._types[x.dtype]
+            here = x.get_device() == self.device.index
+        except (AttributeError, KeyError, ValueError, TypeError):
+            raise ValueError("%s must be a matrix (2-d tensor) of float32, float16 or bfloat16 on %s" % (name, self.device)) from None
+        if not here:
+            raise ValueError("%s must be on %s" % (name, self.device))
+        if dtype is not None and x.dtype != dtype:
+            raise ValueError("%s is %s: must be %s" % (name, x.dtype, dtype))
+        if (rows is not None and n != rows) or (cols is not None and c != cols):
+            raise ValueError("%s is %s: must be (%s, %s)" % (name, (n, c), "any" if rows is None else rows, "any" if cols is None else cols))
+        if n <= 1:
+            ld = c
+        if c < 1 or (one != 1 and c > 1) or ld < c:
             raise ValueError("%s needs at least one column, columns of stride 1 and rows that do not overlap" % name)
-        return x.data_ptr(), self._types[x.dtype], ld
+        return x.data_ptr(), kind, ld, n, c
 
     def _vector(self, x, name, n, dtype=None):
+        """Address of a vector argument, checked; None for None."""
         if x is None:
             return None
-        if not isinstance(x, self.torch.Tensor) or x.device != self.device or x.dtype != (dtype or self.torch.float32) or x.dim() != 1 or x.numel() != n or (n > 1 and x.stride(0) != 1):
-            raise ValueError("%s must be a contiguous %s vector of %d on %s" % (name, dtype or self.torch.float32, n, self.device))
+        dtype = dtype or self.torch.float32
+        try:
+            good = x.dtype == dtype and x.shape == (n,) and (n <= 1 or x.stride(0) == 1) and x.get_device() == self.device.index
+        except AttributeError:
+            good = False
+        if not good:
+            raise ValueError("%s must be a contiguous %s vector of %d on %s" % (name, dtype, n, self.device))
         return x.data_ptr()
 
     def _new(self, n, cols, dtype):
-        """An uninitialised matrix whose rows begin on 16 bytes, and its row stride."""
-        step = 4 if dtype == self.torch.float32 else 8
-        ld = -(-cols // step) * step
-        return self.torch.empty_strided((n, cols), (ld, 1), dtype=dtype, device=self.device), ld
+        """An uninitialised matrix whose rows begin on 16 bytes: (tensor, address, element type, row stride)."""
+        kind = self._types.get(dtype)
+        if kind is None:
+            raise ValueError("%s: must be float32, float16 or bfloat16" % dtype)
+        ld = (cols + 3) & ~3 if kind == _lib.OPAL_F32 else (cols + 7) & ~7
+        t = self.torch
+        y = t.empty((n, cols), dtype=dtype, device=self.device) if ld == cols else t.empty_strided((n, cols), (ld, 1), dtype=dtype, device=self.device)
+        return y, y.data_ptr(), kind, ld
 
     def _run(self, call, tensors, *args):
         """One C call on the engine's stream, ordered with torch's current stream when that is another one."""
+        if self._current(self.device.index) == self._stream:
+            rc = call(self._h, *args)
+            if rc:
+                check(rc, self._h)
+            return
         t = self.torch
         cur = t.cuda.current_stream(self.device)
-        if cur.cuda_stream == self._stream:
-            check(call(self._h, *args), self._h)
-            return
         if t.cuda.is_current_stream_capturing():
             raise RuntimeError("capture on the stream the Engine was created under: its calls run there")
         # (an ExternalStream of handle 0 would be a new stream, not the default one)
@@ -421,85 +445,77 @@ class Engine:
     def layer_norm(self, x, gamma=None, beta=None, eps=1e-5, out_dtype=None, want_stats=False):
         """y = (x - mean) rstd gamma + beta per row (opal_layer_norm).  Returns (y, mean, rstd); mean and rstd are None unless
         want_stats (layer_norm_backward needs them).  out_dtype: of y, default that of x."""
-        t = self.torch
-        px, tx, ldx = self._matrix(x, "x")
-        n, cols = x.shape
+        px, tx, ldx, n, cols = self._matrix(x, "x")
         pg, pb = self._vector(gamma, "gamma", cols), self._vector(beta, "beta", cols)
-        y, ldy = self._new(n, cols, out_dtype or x.dtype)
-        mean, rstd = (t.empty(n, dtype=t.float32, device=self.device), t.empty(n, dtype=t.float32, device=self.device)) if want_stats else (None, None)
-        self._run(lib().opal_layer_norm, (x, gamma, beta, y, mean, rstd), px, tx, ldx, pg, pb, n, cols, eps, y.data_ptr(), self._type(y.dtype), ldy,
-                  mean.data_ptr() if want_stats else None, rstd.data_ptr() if want_stats else None)
+        y, py, ty, ldy = self._new(n, cols, out_dtype or x.dtype)
+        mean = rstd = pm = pr = None
+        if want_stats:
+            t = self.torch
+            mean, rstd = t.empty(n, dtype=t.float32, device=self.device), t.empty(n, dtype=t.float32, device=self.device)
+            pm, pr = mean.data_ptr(), rstd.data_ptr()
+        self._run(self._lib.opal_layer_norm, (x, gamma, beta, y, mean, rstd), px, tx, ldx, pg, pb, n, cols, eps, py, ty, ldy, pm, pr)
         return y, mean, rstd
 
     def layer_norm_backward(self, dy, x, gamma, mean, rstd, out_dtype=None, want_dx=True, want_params=True):
         """The gradients of layer_norm: (dx, dgamma, dbeta) (opal_layer_norm_backward); those not wanted are None.  gamma may be
         None (= 1).  out_dtype: of dx, default that of x."""
         t = self.torch
-        px, tx, ldx = self._matrix(x, "x")
-        n, cols = x.shape
-        pd, td, ldd = self._matrix(dy, "dy", (n, cols))
+        px, tx, ldx, n, cols = self._matrix(x, "x")
+        pd, td, ldd, _, _ = self._matrix(dy, "dy", n, cols)
         pg, pm, pr = self._vector(gamma, "gamma", cols), self._vector(mean, "mean", n), self._vector(rstd, "rstd", n)
         if pm is None or pr is None:
             raise ValueError("mean and rstd of the forward pass are needed (layer_norm(..., want_stats=True))")
-        dx, lddx = self._new(n, cols, out_dtype or x.dtype) if want_dx else (None, 0)
+        dx, px_out, tx_out, lddx = self._new(n, cols, out_dtype or x.dtype) if want_dx else (None, None, 0, 0)
         dg = db = work = None
         size = 0
         if want_params:
             dg, db = t.empty(cols, dtype=t.float32, device=self.device), t.empty(cols, dtype=t.float32, device=self.device)
-            size = lib().opal_layer_norm_backward_workspace(n, cols)
+            size = self._lib.opal_layer_norm_backward_workspace(n, cols)
             work = t.empty(size, dtype=t.uint8, device=self.device)
-        self._run(lib().opal_layer_norm_backward, (dy, x, gamma, mean, rstd, dx, dg, db, work), pd, td, ldd, px, tx, ldx, pg, pm, pr, n, cols,
-                  dx.data_ptr() if want_dx else None, self._type(dx.dtype) if want_dx else 0, lddx, dg.data_ptr() if want_params else None,
-                  db.data_ptr() if want_params else None, work.data_ptr() if want_params else None, size)
+        self._run(self._lib.opal_layer_norm_backward, (dy, x, gamma, mean, rstd, dx, dg, db, work), pd, td, ldd, px, tx, ldx, pg, pm, pr, n, cols, px_out, tx_out,
+                  lddx, dg.data_ptr() if want_params else None, db.data_ptr() if want_params else None, work.data_ptr() if want_params else None, size)
         return dx, dg, db
 
     def linear(self, x, w, bias=None, activation="none", residual=None, out_dtype=None, want_pre=False):
         """y = act(x w^T + bias) + residual (opal_linear): x [n, in] and w [out, in] of one type, bias float32 [out], activation
         none / relu / silu / gelu (tanh form), residual [n, out] of any type.  Returns (y, pre); pre, the value before the
         activation in the type of x (linear_grad_input takes it), is None unless want_pre.  out_dtype: of y, default that of x."""
-        px, tx, ldx = self._matrix(x, "x")
-        n, k = x.shape
-        pw, _, ldw = self._matrix(w, "w", (w.shape[0] if isinstance(w, self.torch.Tensor) else 0, k), x.dtype)
-        m = w.shape[0]
-        pr, tr, ldr = self._matrix(residual, "residual", (n, m)) if residual is not None else (None, 0, 0)
+        px, tx, ldx, n, k = self._matrix(x, "x")
+        pw, _, ldw, m, _ = self._matrix(w, "w", None, k, x.dtype)
+        act = self._activation(activation)
         pb = self._vector(bias, "bias", m)
-        y, ldy = self._new(n, m, out_dtype or x.dtype)
-        pre, ldp = self._new(n, m, x.dtype) if want_pre else (None, 0)
-        self._run(lib().opal_linear, (x, w, bias, residual, y, pre), px, ldx, pw, ldw, tx, pb, self._activation(activation), pr, tr, ldr, n, k, m,
-                  y.data_ptr(), self._type(y.dtype), ldy, pre.data_ptr() if want_pre else None, ldp)
+        pr, tr, ldr, _, _ = self._matrix(residual, "residual", n, m) if residual is not None else (None, 0, 0, 0, 0)
+        y, py, ty, ldy = self._new(n, m, out_dtype or x.dtype)
+        pre, pp, _, ldp = self._new(n, m, x.dtype) if want_pre else (None, None, 0, 0)
+        self._run(self._lib.opal_linear, (x, w, bias, residual, y, pre), px, ldx, pw, ldw, tx, pb, act, pr, tr, ldr, n, k, m, py, ty, ldy, pp, ldp)
         return y, pre
 
     def linear_grad_input(self, dy, w, pre=None, activation="none", residual=None, out_dtype=None):
         """dx = (dy w) act'(pre) + residual (opal_linear_grad_input): dy [n, out] and w [out, in] of one type, pre [n, in] the value
         before the activation that made the product's input (needed unless activation is none), residual [n, in] the gradient
         that reaches the input past the product.  out_dtype: of dx, default that of dy."""
-        pd, td, ldd = self._matrix(dy, "dy")
-        n, m = dy.shape
-        pw, _, ldw = self._matrix(w, "w", (m, w.shape[1] if isinstance(w, self.torch.Tensor) and w.dim() == 2 else 0), dy.dtype)
-        k = w.shape[1]
+        pd, td, ldd, n, m = self._matrix(dy, "dy")
+        pw, _, ldw, _, k = self._matrix(w, "w", m, None, dy.dtype)
         act = self._activation(activation)
         if act and pre is None:
             raise ValueError("an activation's gradient needs pre (linear(..., want_pre=True))")
-        pp, _, ldp = self._matrix(pre, "pre", (n, k), dy.dtype) if act else (None, 0, 0)
-        pr, tr, ldr = self._matrix(residual, "residual", (n, k)) if residual is not None else (None, 0, 0)
-        dx, lddx = self._new(n, k, out_dtype or dy.dtype)
-        self._run(lib().opal_linear_grad_input, (dy, w, pre, residual, dx), pd, ldd, pw, ldw, td, pp, ldp, act, pr, tr, ldr, n, k, m, dx.data_ptr(),
-                  self._type(dx.dtype), lddx)
+        pp, _, ldp, _, _ = self._matrix(pre, "pre", n, k, dy.dtype) if act else (None, 0, 0, 0, 0)
+        pr, tr, ldr, _, _ = self._matrix(residual, "residual", n, k) if residual is not None else (None, 0, 0, 0, 0)
+        dx, px, tx, ldx = self._new(n, k, out_dtype or dy.dtype)
+        self._run(self._lib.opal_linear_grad_input, (dy, w, pre, residual, dx), pd, ldd, pw, ldw, td, pp, ldp, act, pr, tr, ldr, n, k, m, px, tx, ldx)
         return dx
 
     def linear_grad_weight(self, dy, x, want_bias=True):
         """(dw, dbias) = (dy^T x, sum of dy's rows), float32 (opal_linear_grad_weight): dy [n, out] and x [n, in] of one type."""
         t = self.torch
-        px, tx, ldx = self._matrix(x, "x")
-        n, k = x.shape
-        pd, _, ldd = self._matrix(dy, "dy", (n, dy.shape[1] if isinstance(dy, t.Tensor) and dy.dim() == 2 else 0), x.dtype)
-        m = dy.shape[1]
+        px, tx, ldx, n, k = self._matrix(x, "x")
+        pd, _, ldd, _, m = self._matrix(dy, "dy", n, None, x.dtype)
         dw = t.empty((m, k), dtype=t.float32, device=self.device)
         db = t.empty(m, dtype=t.float32, device=self.device) if want_bias else None
-        size = lib().opal_linear_grad_weight_workspace(n, k, m, tx)
-        work = t.empty(size, dtype=t.uint8, device=self.device)
-        self._run(lib().opal_linear_grad_weight, (dy, x, dw, db, work), pd, ldd, px, ldx, tx, n, k, m, dw.data_ptr(), k,
-                  db.data_ptr() if want_bias else None, work.data_ptr(), size)
+        size = self._lib.opal_linear_grad_weight_workspace(n, k, m, tx)
+        work = t.empty(size, dtype=t.uint8, device=self.device) if size else None
+        self._run(self._lib.opal_linear_grad_weight, (dy, x, dw, db, work), pd, ldd, px, ldx, tx, n, k, m, dw.data_ptr(), k,
+                  db.data_ptr() if want_bias else None, work.data_ptr() if size else None, size)
         return dw, db
 
     def softmax_loss(self, scores, labels, scale=1.0, out_dtype=None, want_grad=True):
@@ -507,30 +523,22 @@ class Engine:
         (loss and gradient 0).  Returns (loss float32 [n], scale times the gradient [n, K] or None).  out_dtype: of the gradient,
         default that of scores."""
         t = self.torch
-        ps, ts, lds = self._matrix(scores, "scores")
-        n, K = scores.shape
+        ps, ts, lds, n, K = self._matrix(scores, "scores")
         pl = self._vector(labels, "labels", n, t.int32)
         if pl is None:
             raise ValueError("labels are needed")
         loss = t.empty(n, dtype=t.float32, device=self.device)
-        grad, ldg = self._new(n, K, out_dtype or scores.dtype) if want_grad else (None, 0)
-        self._run(lib().opal_softmax_loss, (scores, labels, loss, grad), ps, ts, lds, n, K, pl, scale, loss.data_ptr(),
-                  grad.data_ptr() if want_grad else None, self._type(grad.dtype) if want_grad else 0, ldg)
+        grad, pg, tg, ldg = self._new(n, K, out_dtype or scores.dtype) if want_grad else (None, None, 0, 0)
+        self._run(self._lib.opal_softmax_loss, (scores, labels, loss, grad), ps, ts, lds, n, K, pl, scale, loss.data_ptr(), pg, tg, ldg)
         return loss, grad
 
     def softmax_class(self, scores):
         """(class int32 [n], 1-based as from predict, its softmax probability float32 [n]) of the highest score of each row."""
         t = self.torch
-        ps, ts, lds = self._matrix(scores, "scores")
-        n, K = scores.shape
+        ps, ts, lds, n, K = self._matrix(scores, "scores")
         cls, prob = t.empty(n, dtype=t.int32, device=self.device), t.empty(n, dtype=t.float32, device=self.device)
-        self._run(lib().opal_softmax_class, (scores, cls, prob), ps, ts, lds, n, K, cls.data_ptr(), prob.data_ptr())
+        self._run(self._lib.opal_softmax_class, (scores, cls, prob), ps, ts, lds, n, K, cls.data_ptr(), prob.data_ptr())
         return cls, prob
-
-    def _type(self, dtype):
-        if dtype not in self._types:
-            raise ValueError("%s: must be float32, float16 or bfloat16" % dtype)
-        return self._types[dtype]
 
     def _activation(self, name):
         if name not in ACTIVATIONS:

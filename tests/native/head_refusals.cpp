@@ -61,8 +61,10 @@ int main()
     want("grad_input dx", opal_linear_grad_input(&ctx, p, 3, p, 4, F, nullptr, 0, 0, nullptr, 0, 0, 2, 4, 3, nullptr, F, 4), E, &ctx, "null dx");
 
     const uint64_t nw = opal_linear_grad_weight_workspace(2, 4, 3, F);
-    want("grad_weight work", opal_linear_grad_weight(&ctx, p, 3, p, 4, F, 2, 4, 3, p, 4, p, p, nw - 1), OPAL_ERANGE, &ctx, "workspace");
-    want("grad_weight nothing", opal_linear_grad_weight(&ctx, p, 3, p, 4, F, 2, 4, 3, nullptr, 4, nullptr, p, nw), E, &ctx, "neither");
+    const uint64_t many = opal_linear_grad_weight_workspace(100000, 4, 3, F);
+    want("grad_weight work", opal_linear_grad_weight(&ctx, p, 3, p, 4, F, 100000, 4, 3, p, 4, p, p, many - 1), OPAL_ERANGE, &ctx, "workspace");
+    want("grad_weight no work", opal_linear_grad_weight(&ctx, p, 3, p, 4, F, 100000, 4, 3, p, 4, p, nullptr, many), OPAL_ERANGE, &ctx, "workspace");
+    want("grad_weight dw", opal_linear_grad_weight(&ctx, p, 3, p, 4, F, 2, 4, 3, nullptr, 4, nullptr, p, nw), E, &ctx, "null dw");
     want("grad_weight dw ld", opal_linear_grad_weight(&ctx, p, 3, p, 4, F, 2, 4, 3, p, 3, p, p, nw), E, &ctx, "row stride of dw");
     want("grad_weight dy", opal_linear_grad_weight(&ctx, nullptr, 3, p, 4, F, 2, 4, 3, p, 4, p, p, nw), E, &ctx, "null dy");
     want("grad_weight type", opal_linear_grad_weight(&ctx, nullptr, 3, nullptr, 4, 5, 0, 4, 3, p, 4, p, p, nw), E, &ctx, "element type");
