@@ -1,0 +1,116 @@
+"""The score head: a trained layer behind the linear model's per-class scores (`train --head H`, `predict`).
+
+The linear model is K independent regressors: its scores are no probabilities and nothing corrects a class that is regularly taken
+for a sister species.  The head reads all K scores s of a fragment,
+
+    z = layer norm(s),   logits = z + W2 gelu(W1 z + b1) + b2,   p = softmax(logits),
+
+and is trained by cross entropy on fragments the linear model has scored, with AdaGrad as the linear learner uses.  It starts as the
+linear model itself (W2 = 0).  The work is Engine.layer_norm, linear, linear_grad_input, linear_grad_weight, softmax_loss and
+softmax_class (hand-written HIP kernels); torch holds the parameters and makes the parameter update, a few passes over them.
+No counterpart in the reference, whose answer is the argmax of the scores (opal.py:449-469)."""
+import os
+import struct
+
+import numpy as np
+
+__all__ = ["ScoreHead", "HEAD_FILE", "batch_scores"]
+
+HEAD_FILE = "vw-model_final.head"        # next to vw-model_final.model
+_HDR = struct.Struct("<8sIII")           # magic, version, K, hidden; then float32 gamma, beta, w1, b1, w2, b2
+_MAGIC = b"OPALHEAD"
+_NAMES = ("gamma", "beta", "w1", "b1", "w2", "b2")
+EPS = 1e-5
+
+
+def batch_scores(engine, batch, reverse, limit=1 << 30):
+    """(first row, scores float32 [rows, K]) of a device batch of fragments, in parts of at most `limit` bytes (one row at least)."""
+    from .engine import DeviceBatch
+    rows = max(1, limit // (4 * engine.K))
+    for lo in range(0, batch.n, rows):
+        hi = min(batch.n, lo + rows)
+        part = DeviceBatch(batch.data, batch.off[lo:hi], batch.len[lo:hi], hi - lo, batch.nbytes)
+        yield lo, engine.predict(part, reverse, want_scores=True)[1]
+
+
+class ScoreHead:
+    def __init__(self, engine, K, hidden, seed=0, params=None):
+        """params: dict of float32 numpy arrays (as load() reads them); else a fresh head of that seed."""
+        t = engine.torch
+        if not (1 <= K <= 1 << 20 and 1 <= hidden <= 1 << 20):
+            raise ValueError("the head needs 1 .. 2^20 classes and hidden units")
+        self.engine, self.K, self.hidden = engine, K, hidden
+        if params is None:
+            w1 = np.random.default_rng(seed).standard_normal((hidden, K), dtype=np.float32) / np.float32(np.sqrt(K))
+            params = dict(gamma=np.ones(K), beta=np.zeros(K), w1=w1, b1=np.zeros(hidden), w2=np.zeros((K, hidden)), b2=np.zeros(K))
+        self.params = {n: t.from_numpy(np.ascontiguousarray(params[n], dtype=np.float32)).to(engine.device) for n in _NAMES}
+        self.grads2 = {n: t.zeros_like(p) for n, p in self.params.items()}             # AdaGrad's sums of squares
+        self._half = {}
+        for n in ("w1", "w2"):                                                         # what the products take: bfloat16, rows on 16 bytes
+            r, c = self.params[n].shape
+            self._half[n] = t.empty_strided((r, c), ((c + 7) & ~7, 1), dtype=t.bfloat16, device=engine.device)
+        self._copy_weights()
+
+    def _copy_weights(self):
+        for n, h in self._half.items():
+            h.copy_(self.params[n])
+
+    def forward(self, scores, for_training=False):
+        """logits float32 [n, K] (and what backward needs) of scores float32 [n, K]."""
+        e, t, p = self.engine, self.engine.torch, self.params
+        z, mean, rstd = e.layer_norm(scores, p["gamma"], p["beta"], eps=EPS, out_dtype=t.bfloat16, want_stats=for_training)
+        h, pre = e.linear(z, self._half["w1"], p["b1"], activation="gelu", want_pre=for_training)
+        logits, _ = e.linear(h, self._half["w2"], p["b2"], residual=z, out_dtype=t.float32)
+        return (logits, (scores, z, mean, rstd, h, pre)) if for_training else logits
+
+    def gradients(self, scores, labels):
+        """(loss float32 [n], dict of the parameters' gradients of the mean loss over the labelled rows' share of n)."""
+        e, t, p = self.engine, self.engine.torch, self.params
+        logits, (scores, z, mean, rstd, h, pre) = self.forward(scores, for_training=True)
+        loss, dl = e.softmax_loss(logits, labels, scale=1.0 / max(scores.shape[0], 1), out_dtype=t.bfloat16)
+        g = {}
+        g["w2"], g["b2"] = e.linear_grad_weight(dl, h)
+        dpre = e.linear_grad_input(dl, self._half["w2"], pre=pre, activation="gelu")
+        g["w1"], g["b1"] = e.linear_grad_weight(dpre, z)
+        dz = e.linear_grad_input(dpre, self._half["w1"], residual=dl)
+        _, g["gamma"], g["beta"] = e.layer_norm_backward(dz, scores, p["gamma"], mean, rstd, want_dx=False)
+        return loss, g
+
+    def train_step(self, scores, labels, rate=0.05):
+        """One AdaGrad step on a batch; labels int32 [n], class ids 1..K (0: no known class).  Returns the loss per row."""
+        loss, g = self.gradients(scores, labels)
+        for n, p in self.params.items():
+            s = self.grads2[n].addcmul_(g[n], g[n])
+            p.addcdiv_(g[n], s.sqrt().add_(1e-8), value=-rate)
+        self._copy_weights()
+        return loss
+
+    def predict(self, scores):
+        """(class int32 [n], 1-based, its probability float32 [n])."""
+        return self.engine.softmax_class(self.forward(scores))
+
+    def save(self, path):
+        with open(path, "wb") as f:
+            f.write(_HDR.pack(_MAGIC, 1, self.K, self.hidden))
+            for n in _NAMES:
+                self.params[n].cpu().numpy().tofile(f)
+
+    @staticmethod
+    def read(path):
+        """(K, hidden, parameters) of a head file; RuntimeError for anything else."""
+        with open(path, "rb") as f:
+            raw = f.read(_HDR.size)
+            if len(raw) < _HDR.size or raw[:8] != _MAGIC:
+                raise RuntimeError("%s is not an opal_amd score head" % path)
+            _, version, K, hidden = _HDR.unpack(raw)
+            if version != 1 or not 1 <= K <= 1 << 20 or not 1 <= hidden <= 1 << 20:
+                raise RuntimeError("unsupported opal_amd score head in %s" % path)
+            shapes = dict(gamma=(K,), beta=(K,), w1=(hidden, K), b1=(hidden,), w2=(K, hidden), b2=(K,))
+            if os.fstat(f.fileno()).st_size != _HDR.size + 4 * sum(int(np.prod(s)) for s in shapes.values()):
+                raise RuntimeError("truncated head file " + path)
+            return K, hidden, {n: np.fromfile(f, dtype=np.float32, count=int(np.prod(shapes[n]))).reshape(shapes[n]) for n in _NAMES}
+
+    @staticmethod
+    def load(engine, path):
+        K, hidden, params = ScoreHead.read(path)
+        return ScoreHead(engine, K, hidden, params=params)

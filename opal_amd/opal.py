@@ -20,6 +20,7 @@ import numpy as np
 from . import drawfrag, fasta2skm, ldpc
 from . import model as model_io
 from .engine import Engine, GenomeSet, Rng, check_geometry, parse_patterns
+from .head import HEAD_FILE, ScoreHead, batch_scores
 from .shard import gather_in_rank_order
 
 __version__ = "1.0.0"
@@ -262,6 +263,9 @@ def train(ref_dir, model_dir, args, engine=None):
         if hierarchical % row_weight != 0:
             raise ValueError("Row weight[{}] must divide into middle hierarchical structure weight [{}].".format(row_weight, hierarchical))
     check_geometry(kmer, row_weight, num_hash + 1)        # before patterns.txt or the model directory are written
+    hidden = getattr(args, "head", 0)
+    if hidden:
+        check_head_options(hidden, args.head_batches, args.head_rows, args.head_rate)
     print("================================================\nTraining using Opal (MI355X-native learner)\n{:%Y-%m-%d %H:%M:%S}\n".format(starttime))
     print("frag_length = {}\ncoverage:       {}\nreverse-complements: {}\nk-mer length:   {}".format(frag_length, coverage, reverse, kmer))
     if hierarchical > 0:
@@ -386,16 +390,63 @@ def train(ref_dir, model_dir, args, engine=None):
                     break
     if w is None:
         w = eng.get_weights()
+    head_file = os.path.join(model_dir, HEAD_FILE)
+    if os.path.exists(head_file):                            # it belongs to the model that was here before
+        os.remove(head_file)
     # --save-resume: the file also carries the accumulators (of the table as trained to the end; with several passes the saved
     # weights may be an earlier pass's, the best on the holdout set) and the number of batches seen
     nnz = model_io.save_model(final_model_file, w, num_labels, bits, g=eng.get_accumulators() if save_resume else None,
                               batches=batches_done + num_batches)
+    if hidden:
+        if multipass:
+            eng.load_weights(w, num_labels, bits)            # the saved regressor, which need not be the last pass's
+        head = train_head(eng, genomes, genome_len, genome_taxid, dico, num_labels, args, log)
+        head.save(head_file)
     log.write("saved %s (%d non-zero weights)\n" % (final_model_file, nnz))
     log.close()
     print("------------------------------------------------\nTotal wall clock runtime (sec): {}\n"
           "================================================".format((datetime.now() - starttime).total_seconds()))
     sys.stdout.flush()
     return 0
+
+
+HEAD_SEED = 1000420       # the head's batches come from draws of their own, so that the linear model's stream is what it is without a head
+
+
+def check_head_options(hidden, batches, rows, rate):
+    if not 1 <= hidden <= 1 << 20:
+        raise ValueError("--head [{}] must lie in 0 .. 2^20".format(hidden))
+    if batches < 1:
+        raise ValueError("--head-batches [{}] must be at least 1".format(batches))
+    if not 1 <= rows <= 1 << 20:
+        raise ValueError("--head-rows [{}] must lie in 1 .. 2^20".format(rows))
+    if not 0 < rate < float("inf"):
+        raise ValueError("--head-rate [{}] must be positive".format(rate))
+
+
+def train_head(eng, genomes, genome_len, genome_taxid, dico, num_labels, args, log):
+    """Trains the score head (opal_amd/head.py) on freshly drawn fragments, scored by the linear model in the engine."""
+    t = eng.torch
+    head = ScoreHead(eng, num_labels, args.head, seed=HEAD_SEED)
+    rng = Rng()
+    for i in range(args.head_batches):
+        print("Drawing fragments for head batch {}".format(i))
+        sys.stdout.flush()
+        vwid, fpos, fgen = draw_training_batch(rng, HEAD_SEED + 1 + i, genome_len, genome_taxid, args.frag_length, args.coverage, dico)
+        if vwid.size and vwid.max() > num_labels:
+            raise ValueError("class id %d exceeds --oaa %d" % (vwid.max(), num_labels))
+        batch = genomes.fragments(fpos, fgen, args.frag_length)
+        labels = t.from_numpy(vwid).to(eng.device)
+        total = t.zeros((), dtype=t.float64, device=eng.device)
+        for lo, scores in batch_scores(eng, batch, args.reverse_complement):
+            for a in range(0, scores.shape[0], args.head_rows):
+                part = scores[a:a + args.head_rows]
+                total += head.train_step(part, labels[lo + a:lo + a + part.shape[0]], args.head_rate).sum(dtype=t.float64)
+        eng.sync()
+        msg = "head batch %d: %d examples, mean loss %.4f" % (i, batch.n, float(total) / max(batch.n, 1))
+        print(msg)
+        log.write(msg + "\n")
+    return head
 
 
 def _next_header(text, start):
@@ -543,6 +594,15 @@ def predict(model_dir, test_dir, predict_dir, args, engine=None, chunk_bytes=Non
     eng = engine or Engine(local)
     eng.set_patterns(pos, kmer)
     hdr = model_io.load_model(model, eng)
+    head = None
+    head_file = os.path.join(model_dir, HEAD_FILE)
+    if os.path.exists(head_file) and not getattr(args, "no_head", False):
+        head = ScoreHead.load(eng, head_file)
+        if head.K != hdr["K"]:
+            raise RuntimeError("%s has %d classes, the model %d" % (head_file, head.K, hdr["K"]))
+    want_prob = bool(getattr(args, "probabilities", False))
+    if want_prob and head is None:
+        raise ValueError("--probabilities needs a model with a score head (train --head)")
     if getattr(args, "dump_vw_text", None) and rank == 0:
         ns = argparse.Namespace(input=fasta, taxid=None, kmer=kmer, dico=None, output=args.dump_vw_text, pattern=pattern_file,
                                 reverse=reverse)
@@ -551,16 +611,23 @@ def predict(model_dir, test_dir, predict_dir, args, engine=None, chunk_bytes=Non
     # every rank scores its own pieces (fragments are independent; no data-path collective); after each
     # round of pieces the class ids are concatenated on rank 0 in piece order = file order
     n_frag, pending = 0, None
+    prob_file = prefix + ".preds.prob"
+    if rank == 0 and os.path.exists(prob_file):                   # an earlier run's: not this run's answers
+        os.remove(prob_file)
+    prob_out = open(prob_file, "w") if rank == 0 and want_prob else None
     out = PredictionFiles(dico, prediction_file, prefix + '.preds.taxid') if rank == 0 else None   # `vw -p` file + vw_class_to_taxid
     try:
         for piece in pieces:
-            cls = None
+            cls = prob = None
             if len(piece):
                 if hasattr(piece, "record_stream"):
                     piece.record_stream(eng.torch.cuda.current_stream(eng.device))
                 batch = eng.ingest_fasta(piece)
-                if batch.n:
+                if batch.n and head is None:
                     cls, _ = eng.predict(batch, reverse)          # asynchronous: the kernel runs while ...
+                elif batch.n:
+                    parts = [head.predict(scores) for _, scores in batch_scores(eng, batch, reverse)]
+                    cls, prob = (eng.torch.cat(v) for v in zip(*parts))
             if pending is not None:
                 out.append(pending)                               # ... the previous round's lines are written
                 pending = None
@@ -569,16 +636,24 @@ def predict(model_dir, test_dir, predict_dir, args, engine=None, chunk_bytes=Non
             if rank == 0:
                 pending = got
                 n_frag += int(got.shape[0])
+            if want_prob:
+                got = gather_in_rank_order(prob.cpu().numpy() if prob is not None else np.zeros(0, dtype=np.float32), dist)
+                if rank == 0:
+                    prob_out.write("".join("%.6f\n" % v for v in got.tolist()))
             del piece
         if pending is not None:
             out.append(pending)
     finally:
         if out is not None:
             out.close()
+        if prob_out is not None:
+            prob_out.close()
     if rank == 0:
         with open(prefix + "_vwps.log", "w") as log:
             log.write("opal_amd scorer: %d fragments, oaa=%d bits=%d, kernel %s, %d rank(s)\n" % (
                 n_frag, hdr["K"], hdr["bits"], eng.predict_kernel_name(), world))
+            if head is not None:
+                log.write("score head: %d hidden units\n" % head.hidden)
         print("------------------------------------------------\nPredicted labels:   {}\nTotal wall clock runtime (sec): {}\n"
               "================================================".format(prefix + '.preds.taxid', (datetime.now() - starttime).total_seconds()))
         sys.stdout.flush()
@@ -641,7 +716,16 @@ def build_parser():
             p.add_argument("--train-mode", choices=sorted(TRAIN_MODES), default=None,
                            help="learner schedule (not in the reference, whose vw process is sequential): deterministic = same model "
                                 "every run (default, or $OPAL_TRAIN_MODE); concurrent = Hogwild; sequential = one wave, slow")
+        if name in ("train", "simulate"):
+            p.add_argument("--head", type=int, default=0, metavar="H",
+                           help="also train a score head of H hidden units behind the per-class scores (not in the reference; 0 = none): "
+                                "predict then answers with it, and can give probabilities")
+            p.add_argument("--head-batches", type=int, default=1, help="freshly sampled batches the head is trained on")
+            p.add_argument("--head-rows", type=int, default=4096, help="fragments per step of the head's learner")
+            p.add_argument("--head-rate", type=float, default=0.05, help="learning rate of the head's learner")
         if name == "predict":
+            p.add_argument("--no-head", action="store_true", help="answer with the linear model alone where the model has a score head")
+            p.add_argument("--probabilities", action="store_true", help="also write the answers' probabilities (needs a score head)")
             p.add_argument("--dump-vw-text", metavar="FILE", default=None,
                            help="debug: also write the VW text lines the reference would pipe to vw (byte-identical)")
         for key in flags:

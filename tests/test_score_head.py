@@ -7,6 +7,7 @@ import ctypes as C
 import os
 import subprocess
 import sys
+import zlib
 
 import numpy as np
 import pytest
@@ -55,7 +56,7 @@ def rows(g, n, cols, t, ld=None, scale=1.0, base=0):
 
 def gen(*key):
     g = torch.Generator()
-    g.manual_seed(abs(hash(key)) % (1 << 31))
+    g.manual_seed(zlib.crc32(repr(key).encode()))
     return g
 
 
@@ -362,7 +363,7 @@ def test_softmax(eng, tx, tg, n, K):
     one = torch.nn.functional.one_hot(labels.long(), K + 1)[:, 1:]
     sc = float(np.float32(scale))
     gref = (p - one) * sc * known[:, None]
-    d = (p * (dz + 6 * U + U * (s64.amax(1, keepdim=True) - s64))[:, :] if False else p * (dz[:, None] + 6 * U + U * spread[:, None])) * sc + 2 * U * sc * one
+    d = p * (dz[:, None] + 6 * U + U * spread[:, None]) * sc + 2 * U * sc * one
     close(grad, gref, d + rounding(gref.abs() + d, tg), "grad")
     cls, prob = eng.softmax_class(s)
     best = s64.amax(1)
