@@ -246,7 +246,7 @@ int opal_eval_counts(opal_ctx *ctx, const int32_t *d_pred, const int32_t *d_ref,
  * alignment; rows of 16-byte alignment are faster for 16- and 32-bit products).  Columns, `in`, `out` and K: 1 .. 2^20; n < 2^31
  * rows, n = 0 is allowed (sums over no rows are zeros).  What lies between two rows is neither used nor written.
  * Parameters, statistics, losses and weight gradients are float32; sums are taken in float32 and a result is rounded once, to
- * its own type.  An output may be one of the inputs only where that is said.  The calls allocate nothing, do not synchronise and can be
+ * its own type.  An output may be one of the inputs only where that is said (whole, in the same place: no other overlap).  The calls allocate nothing, do not synchronise and can be
  * captured into a HIP graph; workspaces are the caller's (16-byte aligned; calls that may overlap need one each), and results are
  * the same bits every time.                                                                                        */
 #define OPAL_F32 0

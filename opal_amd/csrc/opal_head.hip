@@ -66,6 +66,7 @@ struct Norm {
     uint64_t n; int cols; float eps;
     void *y; int y_type; uint64_t ldy;
     float *mean, *rstd;
+    uint64_t first;                            // row of the launch's first block
 };
 
 __device__ __forceinline__ f32x4 param4(const float *p, int col, int left, float none)
@@ -80,7 +81,7 @@ template <class T, int TPR, int NQ, bool NT> __global__ __launch_bounds__(BLOCK)
     constexpr int RPB = BLOCK / TPR;
     const int t = threadIdx.x % TPR;
     const float cols = (float)g.cols;
-    const uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    const uint64_t row = g.first + (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR;
     if (row >= g.n) return;
     f32x4 x[NQ];
     load_row<T, TPR, NQ>((const T *)g.x + row * g.ldx, t, g.cols, 0.f, x);
@@ -336,6 +337,7 @@ struct Softmax {
     void *grad; int grad_type; uint64_t ldg;
     int32_t *out_class; float *out_prob;
     unsigned long long *bad;
+    uint64_t first;                            // row of the launch's first block
 };
 
 // What is known of a row once its maximum and the sum of exponentials are: written by one thread.
@@ -363,7 +365,7 @@ template <class T, int TPR, int NQ, bool NT> __global__ __launch_bounds__(BLOCK)
     Team<TPR> team{red};
     constexpr int RPB = BLOCK / TPR;
     const int t = threadIdx.x % TPR;
-    const uint64_t row = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    const uint64_t row = g.first + (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR;
     if (row >= g.n) return;
     const T *s = (const T *)g.s + row * g.lds;
     f32x4 x[NQ];
@@ -470,16 +472,25 @@ static unsigned row_grid(uint64_t n, int rows_per_block, int cus, int blocks_per
     return (unsigned)std::max<uint64_t>(1, std::min<uint64_t>((n + rows_per_block - 1) / rows_per_block, (uint64_t)cus * blocks_per_cu));
 }
 
-static unsigned blocks_for(uint64_t n, int rows_per_block) { return (unsigned)((n + rows_per_block - 1) / rows_per_block); }
+// A launch has less than 2^32 threads: rows beyond 2^23 blocks are another launch's.  One row a team: fewer blocks that go through
+// the rows took 454 .. 526 us where this takes 423 (250 000 x 1564).
+template <class G, class Launch> static void launch_rows(G g, int rows_per_block, Launch &&launch)
+{
+    const uint64_t most = (uint64_t)rows_per_block << 23;
+    for (g.first = 0; g.first < g.n; g.first += most)
+        launch(g, dim3((unsigned)((std::min(g.n - g.first, most) + rows_per_block - 1) / rows_per_block)));
+}
 
 // Results of more than the 256 MiB that the memory-side cache holds are written past it: 250 000 rows of 1564 in bf16, 423 -> 408 us.
 static bool stream_out(uint64_t n, uint64_t cols, int type) { return n * cols * type_bytes(type) > (256u << 20); }
 
 template <class T> static void run_norm(const Norm &g, int cus, hipStream_t st)
 {
-#define L(TPR, NQ)                                                                                                                  \
-    if (nt) hipLaunchKernelGGL((norm_kernel<T, TPR, NQ, true>), dim3(blocks_for(g.n, BLOCK / TPR)), dim3(BLOCK), 0, st, g);             \
-    else hipLaunchKernelGGL((norm_kernel<T, TPR, NQ, false>), dim3(blocks_for(g.n, BLOCK / TPR)), dim3(BLOCK), 0, st, g)
+#define L(TPR, NQ)                                                                                               \
+    launch_rows(g, BLOCK / TPR, [&](const Norm &q, dim3 blocks) {                                                  \
+        if (nt) hipLaunchKernelGGL((norm_kernel<T, TPR, NQ, true>), blocks, dim3(BLOCK), 0, st, q);                \
+        else hipLaunchKernelGGL((norm_kernel<T, TPR, NQ, false>), blocks, dim3(BLOCK), 0, st, q);                  \
+    })
     const bool nt = stream_out(g.n, g.cols, g.y_type);
     if (g.cols <= BLOCK_COLS) { OPAL_TEAMS(L, g.cols) }
     else hipLaunchKernelGGL(norm_long_kernel<T>, dim3(row_grid(g.n, 1, cus, 2)), dim3(LONG), 0, st, g);
@@ -488,9 +499,11 @@ template <class T> static void run_norm(const Norm &g, int cus, hipStream_t st)
 
 template <class T> static void run_softmax(const Softmax &g, int cus, hipStream_t st)
 {
-#define L(TPR, NQ)                                                                                                                  \
-    if (nt) hipLaunchKernelGGL((softmax_kernel<T, TPR, NQ, true>), dim3(blocks_for(g.n, BLOCK / TPR)), dim3(BLOCK), 0, st, g);          \
-    else hipLaunchKernelGGL((softmax_kernel<T, TPR, NQ, false>), dim3(blocks_for(g.n, BLOCK / TPR)), dim3(BLOCK), 0, st, g)
+#define L(TPR, NQ)                                                                                               \
+    launch_rows(g, BLOCK / TPR, [&](const Softmax &q, dim3 blocks) {                                                  \
+        if (nt) hipLaunchKernelGGL((softmax_kernel<T, TPR, NQ, true>), blocks, dim3(BLOCK), 0, st, q);                \
+        else hipLaunchKernelGGL((softmax_kernel<T, TPR, NQ, false>), blocks, dim3(BLOCK), 0, st, q);                  \
+    })
     const bool nt = g.grad && stream_out(g.n, g.cols, g.grad_type);
     if (g.cols <= BLOCK_COLS) { OPAL_TEAMS(L, g.cols) }
     else hipLaunchKernelGGL(softmax_long_kernel<T>, dim3(row_grid(g.n, 1, cus, 2)), dim3(LONG), 0, st, g);
@@ -542,6 +555,13 @@ static int check_matrix(opal_ctx *ctx, const char *who, const char *name, const 
     return OPAL_OK;
 }
 
+// an output over an input: the same rows, each element written by the thread that has read it
+static int check_in_place(opal_ctx *ctx, const char *who, const char *names, const void *out, int out_type, uint64_t ld_out, const void *in, int in_type, uint64_t ld_in)
+{
+    if (!out || out != in || (out_type == in_type && ld_out == ld_in)) return OPAL_OK;
+    return bad_arg(ctx, who, std::string(names) + " in the same place need the same type and row stride");
+}
+
 static int check_shape(opal_ctx *ctx, const char *who, uint64_t n, uint64_t cols, const char *what)
 {
     if (cols < 1 || cols > MAX_COLS) return bad_arg(ctx, who, std::string("need 1 <= ") + what + " <= 2^20");
@@ -568,10 +588,11 @@ extern "C" int opal_layer_norm(opal_ctx *ctx, const void *d_x, int x_type, uint6
     if (!(eps > 0.f) || !std::isfinite(eps)) return bad_arg(ctx, who, "eps must be positive and finite");
     OPAL_TRY(check_matrix(ctx, who, "x", d_x, x_type, ldx, n, cols));
     OPAL_TRY(check_matrix(ctx, who, "y", d_y, y_type, ldy, n, cols));
+    OPAL_TRY(check_in_place(ctx, who, "x and y", d_y, y_type, ldy, d_x, x_type, ldx));
     if (n == 0) return OPAL_OK;
     OnDevice on(ctx->device);
     OPAL_HIP_CHECK(ctx, on.err);
-    const Norm g{d_x, ldx, d_gamma, d_beta, n, (int)cols, eps, d_y, y_type, ldy, d_mean, d_rstd};
+    const Norm g{d_x, ldx, d_gamma, d_beta, n, (int)cols, eps, d_y, y_type, ldy, d_mean, d_rstd, 0};
     if (x_type == OPAL_F32) run_norm<float>(g, ctx->num_cus, ctx->stream);
     else if (x_type == OPAL_F16) run_norm<f16_t>(g, ctx->num_cus, ctx->stream);
     else run_norm<bf16_t>(g, ctx->num_cus, ctx->stream);
@@ -581,6 +602,7 @@ extern "C" int opal_layer_norm(opal_ctx *ctx, const void *d_x, int x_type, uint6
 
 extern "C" uint64_t opal_layer_norm_backward_workspace(uint64_t n, uint32_t cols)
 {
+    if (n >= MAX_ROWS || cols < 1 || cols > MAX_COLS) return 0;      // what the call refuses
     return norm_back_blocks(n, cols) * 2 * cols * sizeof(float);
 }
 
@@ -594,6 +616,8 @@ extern "C" int opal_layer_norm_backward(opal_ctx *ctx, const void *d_dy, int dy_
     OPAL_TRY(check_matrix(ctx, who, "dy", d_dy, dy_type, lddy, n, cols));
     OPAL_TRY(check_matrix(ctx, who, "x", d_x, x_type, ldx, n, cols));
     OPAL_TRY(check_matrix(ctx, who, "dx", d_dx, dx_type, lddx, n, cols, true));
+    OPAL_TRY(check_in_place(ctx, who, "x and dx", d_dx, dx_type, lddx, d_x, x_type, ldx));
+    OPAL_TRY(check_in_place(ctx, who, "dy and dx", d_dx, dx_type, lddx, d_dy, dy_type, lddy));
     if (n && (!d_mean || !d_rstd)) return bad_arg(ctx, who, "null mean or rstd");
     const bool sums = d_dgamma || d_dbeta;
     const uint64_t blocks = norm_back_blocks(n, cols);
@@ -624,10 +648,11 @@ static int softmax(opal_ctx *ctx, const char *who, const void *d_scores, int typ
     OPAL_TRY(check_shape(ctx, who, n, K, "K"));
     OPAL_TRY(check_matrix(ctx, who, "scores", d_scores, type, ld, n, K));
     OPAL_TRY(check_matrix(ctx, who, "grad", d_grad, grad_type, ldg, n, K, true));
+    OPAL_TRY(check_in_place(ctx, who, "scores and grad", d_grad, grad_type, ldg, d_scores, type, ld));
     if (n == 0) return OPAL_OK;
     OnDevice on(ctx->device);
     OPAL_HIP_CHECK(ctx, on.err);
-    const Softmax g{d_scores, ld, n, (int)K, d_labels, scale, d_loss, d_grad, grad_type, ldg, d_class, d_prob, ctx->d_queue + Q_BAD_LABEL};
+    const Softmax g{d_scores, ld, n, (int)K, d_labels, scale, d_loss, d_grad, grad_type, ldg, d_class, d_prob, ctx->d_queue + Q_BAD_LABEL, 0};
     if (type == OPAL_F32) run_softmax<float>(g, ctx->num_cus, ctx->stream);
     else if (type == OPAL_F16) run_softmax<f16_t>(g, ctx->num_cus, ctx->stream);
     else run_softmax<bf16_t>(g, ctx->num_cus, ctx->stream);
@@ -698,14 +723,37 @@ static bool aligned16(const void *p, uint64_t ld, int type) { return reinterpret
 
 static const char *past(const void *p, uint64_t rows, uint64_t ld, int type) { return p ? (const char *)p + rows * ld * type_bytes(type) : nullptr; }
 
-static int run_rows(opal_ctx *ctx, const char *who, Linear &g, int type, int product)
+// the product without its first `rows` rows
+static Linear behind(const Linear &g, uint64_t rows, int type)
 {
+    Linear q = g;
+    q.M = g.M - rows;
+    q.a = past(g.a, rows, g.lda, type);
+    q.res = past(g.res, rows, g.ldr, g.res_type);
+    q.y = (void *)past(g.y, rows, g.ldy, g.y_type);
+    q.pre_in = past(g.pre_in, rows, g.ldp, type);
+    q.pre_out = (void *)past(g.pre_out, rows, g.ldp, type);
+    return q;
+}
+
+constexpr uint64_t MOST_TILES = 1u << 24;      // of 256 threads in a launch, which has less than 2^32
+
+static int run_rows(opal_ctx *ctx, const char *who, const Linear &product_of, int type, int product)
+{
+    Linear g = product_of;
     OnDevice on(ctx->device);
     OPAL_HIP_CHECK(ctx, on.err);
+    constexpr uint64_t SLICE = 1u << 30;       // rows of a launch: up to 2^23 tiles along M
+    if (g.M > SLICE) {
+        Linear q = g;
+        q.M = SLICE;
+        OPAL_TRY(run_rows(ctx, who, q, type, product));
+        g = behind(g, SLICE, type);
+    }
     const bool dma = aligned16(g.a, g.lda, type) && aligned16(g.b, g.ldb, type);
     const int cus = ctx->num_cus;
     int tile = few_rows(product, g.M, g.N, cus) ? 3 : pick_tile(g.M, g.N, g.K, cus, dma && type != OPAL_F32);
-    if (tile != 3 && tiles_of(g.M, g.N, tile) >= (1ull << 31)) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": too many rows times columns for one call");
+    if (tile != 3 && tiles_of(g.M, g.N, tile) >= MOST_TILES) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": too many rows times columns for one call");
     g.splits = 1;
     g.ksplit = g.K;
     auto run = [&](Linear &q, int t) {
@@ -726,14 +774,7 @@ static int run_rows(opal_ctx *ctx, const char *who, Linear &g, int type, int pro
         Linear q = g;
         q.M = rows;
         OPAL_HIP_CHECK(ctx, run(q, 2));
-        q = g;
-        q.M = g.M - rows;
-        q.a = past(g.a, rows, g.lda, type);
-        q.res = past(g.res, rows, g.ldr, g.res_type);
-        q.y = (void *)past(g.y, rows, g.ldy, g.y_type);
-        q.pre_in = past(g.pre_in, rows, g.ldp, type);
-        q.pre_out = (void *)past(g.pre_out, rows, g.ldp, type);
-        g = q;
+        g = behind(g, rows, type);
         tile = few_rows(product, g.M, g.N, cus) ? 3 : pick_tile(g.M, g.N, g.K, cus, false);
     }
     OPAL_HIP_CHECK(ctx, run(g, tile));
@@ -755,6 +796,8 @@ extern "C" int opal_linear(opal_ctx *ctx, const void *d_x, uint64_t ldx, const v
     OPAL_TRY(check_matrix(ctx, who, "y", d_y, y_type, ldy, n, out));
     OPAL_TRY(check_matrix(ctx, who, "pre", d_pre, type, ldp, n, out, true));
     if (n == 0) return OPAL_OK;
+    OPAL_TRY(check_in_place(ctx, who, "the residual and y", d_y, y_type, ldy, d_res, res_type, ldr));
+    if (d_y == d_x || d_y == d_w || d_y == d_pre || (d_pre && (d_pre == d_x || d_pre == d_w || d_pre == d_res))) return bad_arg(ctx, who, "y and pre need places of their own");
     Linear g{};
     g.a = (const char *)d_x; g.lda = ldx; g.b = (const char *)d_w; g.ldb = ldw;
     g.M = n; g.N = out; g.K = in;
@@ -781,6 +824,8 @@ extern "C" int opal_linear_grad_input(opal_ctx *ctx, const void *d_dy, uint64_t 
     OPAL_TRY(check_matrix(ctx, who, "the residual", d_res, res_type, ldr, n, in, true));
     OPAL_TRY(check_matrix(ctx, who, "dx", d_dx, dx_type, lddx, n, in));
     if (n == 0) return OPAL_OK;
+    OPAL_TRY(check_in_place(ctx, who, "the residual and dx", d_dx, dx_type, lddx, d_res, res_type, ldr));
+    if (d_dx == d_dy || d_dx == d_w || d_dx == d_pre) return bad_arg(ctx, who, "dx needs a place of its own");
     Linear g{};
     g.a = (const char *)d_dy; g.lda = lddy; g.b = (const char *)d_w; g.ldb = ldw;
     g.M = n; g.N = in; g.K = out;
@@ -809,7 +854,7 @@ static Splits weight_splits(uint64_t n, uint32_t in, uint32_t out, int type)
 
 extern "C" uint64_t opal_linear_grad_weight_workspace(uint64_t n, uint32_t in, uint32_t out, int type)
 {
-    if (!type_ok(type)) return 0;
+    if (!type_ok(type) || n >= MAX_ROWS || in < 1 || out < 1 || in > MAX_COLS || out > MAX_COLS) return 0;      // what the call refuses
     const Splits s = weight_splits(n, in, out, type);
     return s.splits > 1 ? s.splits * ((uint64_t)in * out + out) * sizeof(float) : 0;
 }
@@ -820,7 +865,7 @@ namespace opal_head {
 __global__ __launch_bounds__(BLOCK) void sum_splits_kernel(const float *part, const float *rows, uint32_t splits, uint64_t each, uint32_t cols, uint32_t out,
                                                            float *dw, uint64_t ld, float *db)
 {
-    const uint64_t quads = dw ? (each + 3) / 4 : 0, all = quads + (db ? out : 0);
+    const uint64_t quads = (each + 3) / 4, all = quads + (db ? out : 0);
     for (uint64_t i = (uint64_t)blockIdx.x * BLOCK + threadIdx.x; i < all; i += (uint64_t)gridDim.x * BLOCK) {
         if (i >= quads) {
             const uint64_t r = i - quads;
@@ -873,7 +918,7 @@ extern "C" int opal_linear_grad_weight(opal_ctx *ctx, const void *d_dy, uint64_t
     Linear g{};
     g.a = (const char *)d_dy; g.lda = lddy; g.b = (const char *)d_x; g.ldb = ldx;
     g.M = out; g.N = in; g.K = n;
-    if (tiles_of(g.M, g.N, tile) * s.splits >= (1ull << 31)) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": in times out is too large for one call");
+    if (tiles_of(g.M, g.N, tile) * s.splits >= MOST_TILES) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": in times out is too large for one call");
     set_tiles(g, tile);
     g.splits = (uint32_t)s.splits;
     g.ksplit = s.rows;

@@ -75,6 +75,30 @@ int main()
     want("loss K", opal_softmax_loss(&ctx, p, F, 4, 2, 0, lab, 1.f, p, p, F, 3), E, &ctx, "K");
     want("class out", opal_softmax_class(&ctx, p, F, 4, 2, 4, nullptr, p), E, &ctx, "d_out_class");
     want("class ctx", opal_softmax_class(nullptr, p, F, 4, 2, 4, lab, p), E, nullptr, "null ctx");
+
+    // an output over an input: with another type or row stride, or where no input may be overwritten
+    const int H = OPAL_BF16;
+    float *q = buf + 32;
+    want("norm over x", opal_layer_norm(&ctx, p, F, 4, nullptr, nullptr, 2, 4, 1e-5f, p, H, 4, nullptr, nullptr), E, &ctx, "same place");
+    want("norm over x ld", opal_layer_norm(&ctx, p, F, 4, nullptr, nullptr, 2, 4, 1e-5f, p, F, 5, nullptr, nullptr), E, &ctx, "same place");
+    want("back over x", opal_layer_norm_backward(&ctx, q, F, 4, p, F, 4, p, p, p, 2, 4, p, F, 8, p, p, p, nb), E, &ctx, "same place");
+    want("back over dy", opal_layer_norm_backward(&ctx, q, F, 4, p, F, 4, p, p, p, 2, 4, q, H, 4, p, p, p, nb), E, &ctx, "same place");
+    want("linear over res", opal_linear(&ctx, p, 4, p + 8, 4, F, nullptr, 0, q, F, 4, 2, 4, 3, q, F, 3, nullptr, 0), E, &ctx, "same place");
+    want("linear over x", opal_linear(&ctx, p, 4, p + 8, 4, F, nullptr, 0, nullptr, 0, 0, 2, 4, 3, p, F, 3, nullptr, 0), E, &ctx, "own");
+    want("linear over w", opal_linear(&ctx, p, 4, p + 8, 4, F, nullptr, 0, nullptr, 0, 0, 2, 4, 3, p + 8, F, 3, nullptr, 0), E, &ctx, "own");
+    want("linear pre over y", opal_linear(&ctx, p, 4, p + 8, 4, F, nullptr, 0, nullptr, 0, 0, 2, 4, 3, q, F, 3, q, 3), E, &ctx, "own");
+    want("grad_input over dy", opal_linear_grad_input(&ctx, p, 3, q, 4, F, nullptr, 0, 0, nullptr, 0, 0, 2, 4, 3, p, F, 4), E, &ctx, "own");
+    want("grad_input over res", opal_linear_grad_input(&ctx, p, 3, p + 8, 4, F, nullptr, 0, 0, q, F, 4, 2, 4, 3, q, H, 4), E, &ctx, "same place");
+    want("loss over scores", opal_softmax_loss(&ctx, p, F, 4, 2, 4, lab, 1.f, q, p, H, 4), E, &ctx, "same place");
+
+    // sizes that the calls refuse need no workspace
+    const uint32_t none = 0, big = (1u << 20) + 1;
+    if (opal_linear_grad_weight_workspace(100, none, 3, F) || opal_linear_grad_weight_workspace(100, 3, none, F) || opal_linear_grad_weight_workspace(100, big, 3, F) ||
+        opal_linear_grad_weight_workspace(100, 3, big, H) || opal_linear_grad_weight_workspace(~0ull, 3, 3, F) || opal_layer_norm_backward_workspace(100, none) ||
+        opal_layer_norm_backward_workspace(100, big) || opal_layer_norm_backward_workspace(~0ull, 4)) {
+        printf("a workspace for sizes that are refused\n");
+        failures++;
+    }
     if (failures) return 1;
     printf("head refusals: ok\n");
     return 0;

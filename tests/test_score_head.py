@@ -568,6 +568,39 @@ def test_rows_beyond_32_bits(eng):
 
 # ------------------------------------------------------------------------------ refusals
 @pytest.mark.gpu
+def test_more_rows_than_one_launch_holds(eng):
+    """2^28 + 17 rows for teams of 16 lanes, 2^30 + 300 for a product: the results of the rows around the seam and at both ends are
+    those of the same rows alone (a row's arithmetic does not look at the others)."""
+    n = (1 << 28) + 17
+    x = torch.empty(n, 2, dtype=BF16, device="cuda")
+    x.view(torch.int32)[:, 0] = torch.arange(n, dtype=torch.int32, device="cuda") * 40503 & 0x3fff3fff        # finite pairs of bf16
+    gamma, beta = torch.tensor([0.5, 2.0], device="cuda"), torch.tensor([0.25, -1.0], device="cuda")
+    parts = [(0, 3000), ((1 << 28) - 100, n)]
+    y, mean, rstd = eng.layer_norm(x, gamma, beta, want_stats=True)
+    for a, b in parts:
+        py, pm, pr = eng.layer_norm(x[a:b], gamma, beta, want_stats=True)
+        assert torch.equal(y[a:b], py) and torch.equal(mean[a:b], pm) and torch.equal(rstd[a:b], pr)
+    del y, mean, rstd
+    labels = (torch.arange(n, dtype=torch.int32, device="cuda") % 3)
+    loss, grad = eng.softmax_loss(x, labels)
+    cls, prob = eng.softmax_class(x)
+    for a, b in parts:
+        pl, pg = eng.softmax_loss(x[a:b], labels[a:b])
+        pc, pp = eng.softmax_class(x[a:b])
+        assert torch.equal(loss[a:b], pl) and torch.equal(grad[a:b, :], pg) and torch.equal(cls[a:b], pc) and torch.equal(prob[a:b], pp)
+    del x, loss, grad, cls, prob, labels
+    n = (1 << 30) + 300
+    x = torch.empty(n, 1, dtype=BF16, device="cuda")
+    x.copy_((torch.arange(n, dtype=torch.int32, device="cuda") % 251 - 125)[:, None])
+    w, bias = torch.tensor([[0.75]], dtype=BF16, device="cuda"), torch.tensor([0.5], device="cuda")
+    y = torch.empty_strided((n, 1), (1, 1), dtype=BF16, device="cuda")
+    from opal_amd._lib import check
+    check(eng._lib.opal_linear(eng._h, x.data_ptr(), 1, w.data_ptr(), 1, 2, bias.data_ptr(), 0, None, 0, 0, n, 1, 1, y.data_ptr(), 2, 1, None, 0), eng._h)
+    for a, b in [(0, 3000), ((1 << 30) - 200, n)]:                  # 0.75 k + 0.5: exact in 32 bits, one rounding
+        assert torch.equal(y[a:b], (x[a:b].float() * 0.75 + 0.5).to(BF16))
+
+
+@pytest.mark.gpu
 def test_engine_refuses(eng):
     x, w = torch.randn(4, 8, device="cuda"), torch.randn(6, 8, device="cuda")
     lab = torch.ones(4, dtype=torch.int32, device="cuda")
