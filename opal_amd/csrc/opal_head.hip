@@ -686,21 +686,27 @@ static hipError_t launch(const Linear &g, int type, int product, int tile, bool 
     return launch_linear<bf16_t>(g, product, tile, dma, st);
 }
 
-constexpr int TILE[] = {64, 128, 256};
+constexpr int TILE_M[] = {64, 128, 256, 0, 128}, TILE_N[] = {64, 128, 256, 0, 256};
 
-static uint64_t tiles_of(uint64_t M, uint64_t N, int tile) { return ((M + TILE[tile] - 1) / TILE[tile]) * ((N + TILE[tile] - 1) / TILE[tile]); }
+static uint64_t tiles_of(uint64_t M, uint64_t N, int tile) { return ((M + TILE_M[tile] - 1) / TILE_M[tile]) * ((N + TILE_N[tile] - 1) / TILE_N[tile]); }
 
-// Larger tiles read fewer bytes for the same sums, smaller ones leave fewer CUs idle.
-//   128 x 128 from 1.5 tiles a CU on: 4096 x 512 x 1564 (416 tiles) 14.4 us against 15.1 with 64 x 64, 16384 x 1564 x 512 (512) 34.5 against
-//   49.3; below it 4096 x 1564 x 512 (128) 21.8 against 12.2, 32768 x 356 x 128 (256) 11.5 against 10.7.  32-bit types the same: 65536 x 356 x 100 (512) 58.1
-//   against 57.2, 16384 x 1564 x 512 (512) 201 against 213.
-//   256 x 256 (16-bit types, aligned) from one tile a CU on, four where the sums are short and its epilogue shows: 32768 x 1564 x 512 (256) 50.9
-//   us against 68.0 with 128 x 128, 65536 x 512 x 1564 (1792) 145 against 177; below it 16384 x 1564 x 512 (128) 36.6 against 34.5, 16384 x 512 x 1564
-//   (448) 59.0 against 49.6, 65536 x 356 x 128 (256) 19.3 against 17.6.
-static int pick_tile(uint64_t M, uint64_t N, uint64_t K, int cus, bool big)
+// Larger tiles read fewer bytes for the same sums, smaller ones leave fewer CUs idle (us; M x N x K):
+//   128 x 128 instead of 64 x 64 from 1.5 tiles a CU on: 4096 x 512 x 1564 (416 tiles) 14.4 against 15.1, 16384 x 1564 x 512 (512) 34.5 against
+//   49.3; below it 4096 x 1564 x 512 (128) 21.8 against 12.2, 32768 x 356 x 128 (256) 11.5 against 10.7.  32-bit types the same.
+// 16-bit types, aligned:
+//   256 x 256 for sums of 1024 on from one tile a CU on: 32768 x 512 x 1564 (256) 51 against 59 with 128 x 256 and 70 with 128 x 128; below it 16384 x 512
+//   x 1564 (128) 38 against 32 and 35.  For sums of 256 on an input gradient the same (32768 x 512 x 256: 17.5 against 22.3; sums of 128 82 against 73);
+//   a forward product, which has 128 x 256 tiles too, from four on: 250 000 x 355 x 256 (1954) 106 against 110, 100 000 x 1563 x 256 140
+//   against 169; below it 100 000 x 512 x 512 (782) 76 against 70, 32768 x 1564 x 512 (896) 72 against 68.
+//   128 x 256 (forward, more than 128 columns) from 3/4 of a tile a CU on: 250 000 x 355 x 128 66 against 82 with 256 x 256 and 104 with 128 x 128, 4096 x
+//   1564 x 512 (224) 14.1 against 15.5; below it 4099 x 512 x 355 (66) 12.2 against 10.9, 16384 x 200 x 200 (128) 10.9 against 7.7.
+// large: the last two may take it; whole: the first of them too.
+static int pick_tile(int product, uint64_t M, uint64_t N, uint64_t K, int cus, bool large, bool whole)
 {
-    if (big && tiles_of(M, N, 2) >= (uint64_t)cus * (K >= 1024 ? 1 : 4)) return 2;
-    return tiles_of(M, N, 1) * 2 >= (uint64_t)cus * 3 ? 1 : 0;
+    const uint64_t c = cus;
+    if (large && whole && K >= 256 && tiles_of(M, N, 2) >= (product == FWD && K < 1024 ? 4 * c : c)) return 2;
+    if (large && product == FWD && N > 128 && tiles_of(M, N, 4) * 4 >= 3 * c) return 4;
+    return tiles_of(M, N, 1) * 2 >= 3 * c ? 1 : 0;
 }
 
 // The kernel for few rows, while its blocks (64 x 16 results, all of k) find a CU each: 64 x 1564 x 512 in 8.1 us against 10.3 with
@@ -714,8 +720,8 @@ static bool few_rows(int product, uint64_t M, uint64_t N, int cus)
 
 static void set_tiles(Linear &g, int tile)
 {
-    g.tm = (uint32_t)((g.M + TILE[tile] - 1) / TILE[tile]);
-    g.tn = (uint32_t)((g.N + TILE[tile] - 1) / TILE[tile]);
+    g.tm = (uint32_t)((g.M + TILE_M[tile] - 1) / TILE_M[tile]);
+    g.tn = (uint32_t)((g.N + TILE_N[tile] - 1) / TILE_N[tile]);
 }
 
 // 16-byte chunks straight into LDS need matrices and rows that begin on 16 bytes
@@ -752,7 +758,9 @@ static int run_rows(opal_ctx *ctx, const char *who, const Linear &product_of, in
     }
     const bool dma = aligned16(g.a, g.lda, type) && aligned16(g.b, g.ldb, type);
     const int cus = ctx->num_cus;
-    int tile = few_rows(product, g.M, g.N, cus) ? 3 : pick_tile(g.M, g.N, g.K, cus, dma && type != OPAL_F32);
+    // (the two kernels for large products write 32 bits or the operands' type, and read such a residual)
+    const bool large = dma && type != OPAL_F32 && (g.y_type == OPAL_F32 || g.y_type == type) && (!g.res || g.res_type == OPAL_F32 || g.res_type == type);
+    int tile = few_rows(product, g.M, g.N, cus) ? 3 : pick_tile(product, g.M, g.N, g.K, cus, large, true);
     if (tile != 3 && tiles_of(g.M, g.N, tile) >= MOST_TILES) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": too many rows times columns for one call");
     g.splits = 1;
     g.ksplit = g.K;
@@ -768,14 +776,14 @@ static int run_rows(opal_ctx *ctx, const char *who, const Linear &product_of, in
     };
     // 256 x 256 tiles come in rounds of one a CU.  A last round of up to a quarter of the CUs goes to smaller tiles instead, in a
     // launch of its own: 100 000 x 1564 x 512 (3.05 rounds) 239 -> 220 us; with two fifths, 60 001 x 512 x 1563 (6.43), 312 -> 328.
-    const uint64_t tn = (g.N + TILE[2] - 1) / TILE[2], tiles = tiles_of(g.M, g.N, 2), rounds = tiles / cus;
-    const uint64_t rows = rounds * cus / tn * TILE[2];
-    if (tile == 2 && rounds && rows < g.M && (tiles - rows / TILE[2] * tn) * 4 <= (uint64_t)cus) {
+    const uint64_t tn = (g.N + TILE_M[2] - 1) / TILE_M[2], tiles = tiles_of(g.M, g.N, 2), rounds = tiles / cus;
+    const uint64_t rows = rounds * cus / tn * TILE_M[2];
+    if (tile == 2 && rounds && rows < g.M && (tiles - rows / TILE_M[2] * tn) * 4 <= (uint64_t)cus) {
         Linear q = g;
         q.M = rows;
         OPAL_HIP_CHECK(ctx, run(q, 2));
         g = behind(g, rows, type);
-        tile = few_rows(product, g.M, g.N, cus) ? 3 : pick_tile(g.M, g.N, g.K, cus, false);
+        tile = few_rows(product, g.M, g.N, cus) ? 3 : pick_tile(product, g.M, g.N, g.K, cus, large, false);
     }
     OPAL_HIP_CHECK(ctx, run(g, tile));
     return OPAL_OK;

@@ -530,7 +530,7 @@ template <class T, int P, int TM> __global__ __launch_bounds__(FEW_WAVES * WAVE)
 }
 
 // The launch of one product in one element type (opal_linear_{f32,f16,bf16}.hip); tile: 0 = 64 x 64, 1 = 128 x 128, 2 = 256 x 256
-// (16-bit types on the aligned path only), 3 = few rows (g.few x 16).
+// (16-bit types on the aligned path only), 3 = few rows (g.few x 16), 4 = 128 x 256 (FWD, as 2).
 template <class T> hipError_t launch_linear(const Linear &g, int product, int tile, bool dma, hipStream_t stream);
 
 #define OPAL_LINEAR_CASE(T, P, TILE, BM, BN, WM, WN, D)                                                                              \

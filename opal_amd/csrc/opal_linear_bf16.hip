@@ -1,9 +1,10 @@
 // The matrix products of the score head for elements of type bf16_t (opal_linear.h).
-#include "opal_linear_big.h"
+#include "opal_linear_pair.h"
 
 namespace opal_head {
 template <> hipError_t launch_linear<bf16_t>(const Linear &g, int product, int tile, bool dma, hipStream_t stream)
 {
+    if (tile == 4 && dma && product == FWD) return launch_pair<bf16_t>(g, stream);
     if (tile == 2 && dma) return launch_big<bf16_t>(g, product, stream);
     OPAL_LINEAR_CASES(bf16_t, FWD)
     OPAL_LINEAR_CASES(bf16_t, GIN)

@@ -1,7 +1,9 @@
 // The product kernel for large 16-bit matrices on 16 bytes (opal_linear.h has the products, the operands' layouts and the kernel
 // for everything else): 256 x 256 tiles, eight waves of 128 x 64, one block per CU that stays for all its tiles, steps of 32 k.
 //
-// What bounds it is the matrix pipe, so everything else runs beside it.
+// What bounds it: the matrix pipe and LDS, which are asked for nearly the same time (a step of 32 k: 1024 cycles; 96 KB read at 128 bytes a
+// cycle, 32 KB arriving from memory at 64), so everything else runs beside them.  Sums of the hidden layer's product (250 000 x 512 x 1564):
+// 1613 TFLOP/s without requests, 1146 with them, 1004 with the epilogue (399 us).
 //   - Waves 0 .. 3 and 4 .. 7 share the four SIMDs and take turns: while one half multiplies (16 MFMAs, its requests for chunks in
 //     between), the other reads its next fragments, with a barrier at each change; half 1 runs one change behind half 0.
 //   - Chunks come straight into LDS, well ahead and over the ends of tiles.  Half 0 asks for A's, half 1 for B's: vmcnt counts a
@@ -12,42 +14,6 @@
 #include "opal_linear.h"
 
 namespace opal_head {
-
-// Four neighbouring elements of a matrix whose type is known at run time, as they lie in memory: loads can be started well
-// before they are used.
-struct RawQuad { uint32_t w[4]; };
-__device__ __forceinline__ RawQuad load_raw(const void *base, int type, uint64_t at, int m)
-{
-    RawQuad r = {{0, 0, 0, 0}};
-    if (m >= 4) {
-        if (type == OPAL_F32) {
-            const Quad<float> q = *reinterpret_cast<const Quad<float> *>((const float *)base + at);
-            __builtin_memcpy(r.w, &q, 16);
-        } else {
-            const Quad<f16_t> q = *reinterpret_cast<const Quad<f16_t> *>((const f16_t *)base + at);
-            __builtin_memcpy(r.w, &q, 8);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 3; i++)
-            if (i < m) {
-                if (type == OPAL_F32) r.w[i] = ((const uint32_t *)base)[at + i];
-                else r.w[i / 2] |= (uint32_t)((const uint16_t *)base)[at + i] << (16 * (i & 1));
-            }
-    }
-    return r;
-}
-__device__ __forceinline__ f32x4 decode(const RawQuad &r, int type)
-{
-    if (type == OPAL_F32) return f32x4{__builtin_bit_cast(float, r.w[0]), __builtin_bit_cast(float, r.w[1]), __builtin_bit_cast(float, r.w[2]), __builtin_bit_cast(float, r.w[3])};
-    if (type == OPAL_BF16)
-        return f32x4{__builtin_bit_cast(float, r.w[0] << 16), __builtin_bit_cast(float, r.w[0] & 0xffff0000u), __builtin_bit_cast(float, r.w[1] << 16),
-                     __builtin_bit_cast(float, r.w[1] & 0xffff0000u)};
-    struct H { f16_t v[4]; };
-    H h;
-    __builtin_memcpy(&h, r.w, 8);
-    return f32x4{(float)h.v[0], (float)h.v[1], (float)h.v[2], (float)h.v[3]};
-}
 
 constexpr int BIG = 256, BIG_THREADS = 512, BIG_STEP = 32;
 
@@ -97,7 +63,7 @@ template <int P, bool IS_A> struct Ring {
         }
     }
 };
-constexpr int BIG_TURN = 8 * 64 * 4;           // bytes: a wave's turning place
+constexpr int RES16 = 1, RES32 = 2;            // kinds of residual: the operands' type, 32 bits
 
 // the k of a KC fragment behind the matrix's edge: `left` values of k from the fragment's first on are the matrix's
 __device__ __forceinline__ s16x8 keep_k(s16x8 f, int left)
@@ -228,74 +194,38 @@ template <int P> struct Feed {
 };
 
 // ------------------------------------------------------------------------------------------------ epilogue
-template <class T> __device__ __forceinline__ constexpr int own_type() { return __is_same(T, f16_t) ? OPAL_F16 : OPAL_BF16; }
 
-// Tiles at the edge of N that cut a group of eight columns, and the rarer mixes of types: the wave's 128 x 64 results, eight rows at
-// a time (slice = 4 i + quarter) through its own 2 KB of LDS, one element after the other: little code, since what a tile executes
-// has to stay in the instruction cache.
-__device__ __forceinline__ float load1(const void *base, int type, uint64_t at)
-{
-    return type == OPAL_F32 ? ((const float *)base)[at] : type == OPAL_F16 ? (float)((const f16_t *)base)[at] : (float)((const bf16_t *)base)[at];
-}
-__device__ __forceinline__ void store1(void *base, int type, uint64_t at, float v)
-{
-    if (type == OPAL_F32) ((float *)base)[at] = v;
-    else if (type == OPAL_F16) ((f16_t *)base)[at] = (f16_t)v;
-    else ((bf16_t *)base)[at] = (bf16_t)v;
-}
-template <class T, int P, int ACT>
-__device__ __forceinline__ void epilogue_any(const Linear &g, const BigItem &c, const f32x16 (&acc)[4][2], float *turn, int wm, int wn, int rot)
-{
-    constexpr int own = own_type<T>();
-    const int lane = threadIdx.x & 63;
-    const uint32_t n = c.n0 + wn + lane, m0 = c.m0 + wm;
-    float bias = P == FWD && g.bias && n < g.N ? g.bias[n] : 0.f;
-    asm volatile("" : "+v"(bias));             // arrives here: were it left to its use, the main loop would be made to wait for it
-#pragma unroll 1
-    for (int s = 0; s < 16; s++) {
-        const int r = lane & 7;
-        if (((lane >> 3) & 3) == (s & 3)) {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if ((s >> 2) == i)
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-#pragma unroll
-                        for (int q = 0; q < 4; q++)
-                            *reinterpret_cast<f32x4 *>(turn + r * 64 + (((j * 8 + q * 2 + (lane >> 5)) ^ (r * 2)) * 4)) =
-                                f32x4{acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]};
-        }
-        wave_order();
-#pragma unroll 2
-        for (int row = 0; row < 8; row++) {                    // a lane a column
-            const uint64_t m = m0 + (((s >> 2) + rot) & 3) * 32 + (s & 3) * 8 + row;
-            float v = turn[row * 64 + (((lane >> 2) ^ (row * 2)) * 4) + (lane & 3)];
-            if (m < g.M && n < g.N) {
-                if (P == GIN && ACT) v *= act_slope(load1(g.pre_in, own, m * g.ldp + n), ACT);
-                if (P == FWD) {
-                    v += bias;
-                    if (g.pre_out) store1(g.pre_out, own, m * g.ldp + n, v);
-                    v = act_value(v, ACT);
-                }
-                if (P != GWT && g.res) v += load1(g.res, g.res_type, m * g.ldr + n);
-                store1(g.y, g.y_type, c.split * g.y_split + m * g.ldy + n, v);
-            }
-        }
-        wave_order();
-    }
-}
-
-// Eight columns of a row in a 16-bit type, 16 bytes: the lanes l and l + 32 hold columns 0..3 and 4..7 of the groups x and y (of the
-// same row); afterwards l holds the eight of x and l + 32 those of y.
-__device__ __forceinline__ u32x4 join_halves(uint32_t x0, uint32_t x1, uint32_t y0, uint32_t y1)
+// An accumulator's 32 x 32 results: a lane holds row l % 32 and of each group of eight columns four, 16 bytes (8 in 16 bits) here and
+// there.  What a wave writes at once should be long pieces of rows, so two exchanges of lanes put columns where rows were:
+//   by 16 lanes: a lane holds rows l % 16 and l % 16 + 16, and four columns of each 16: 4 lanes make 64 bytes of a row in 32 bits
+//   by 32 lanes (16-bit results only): eight columns of 32: 4 lanes make 64 bytes of a row
+template <int LANES> __device__ __forceinline__ void exchange(uint32_t &x, uint32_t &y)
 {
 #ifdef __HIP_DEVICE_COMPILE__
-    const auto a = __builtin_amdgcn_permlane32_swap(x0, y0, false, false);
-    const auto b = __builtin_amdgcn_permlane32_swap(x1, y1, false, false);
-    return u32x4{a[0], b[0], a[1], b[1]};
-#else
-    return u32x4{x0, x1, y0, y1};
+    if constexpr (LANES == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+        x = r[0];
+        y = r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+        x = r[0];
+        y = r[1];
+    }
 #endif
+}
+// v[8 u + 4 R + e] afterwards: row 16 R + l % 16, column 16 u + 8 (l / 16 % 2) + 4 (l / 32) + e
+__device__ __forceinline__ void turn16(f32x16 &v)
+{
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float a = v[u * 8 + e], b = v[u * 8 + 4 + e];
+            uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+            exchange<16>(x, y);
+            v[u * 8 + e] = __builtin_bit_cast(float, x);
+            v[u * 8 + 4 + e] = __builtin_bit_cast(float, y);
+        }
 }
 template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b)
 {
@@ -303,95 +233,123 @@ template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b)
     return __builtin_bit_cast(uint32_t, h);
 }
 struct __attribute__((packed, aligned(2))) Any16 { uint32_t w[4]; };
-struct __attribute__((packed, aligned(2))) Any8 { uint32_t w[2]; };
 
-// Whole groups of eight columns, results in 32 bits or the operands' type: 32 x 32 results at a time, straight from the accumulators.
-// A lane holds row l % 32 and, of a group of eight columns, four; 16-bit results are joined to 16 bytes a lane.  What is read is
-// asked for one block ahead.
-template <class T> __device__ __forceinline__ void store_joined(void *to, uint64_t at, bool in, const f32x16 &a, int qq)
+// row R's eight columns from 16 (l / 32) + 8 (l / 16 % 2) on, of a turned block; `left` of them the matrix's
+template <class T> __device__ __forceinline__ void store_joined(void *to, uint64_t at, int left, const f32x16 &v, int R)
 {
-    const u32x4 o = join_halves(pack2<T>(a[qq * 8], a[qq * 8 + 1]), pack2<T>(a[qq * 8 + 2], a[qq * 8 + 3]), pack2<T>(a[qq * 8 + 4], a[qq * 8 + 5]),
-                                pack2<T>(a[qq * 8 + 6], a[qq * 8 + 7]));
-    if (in) *reinterpret_cast<Any16 *>((T *)to + at) = __builtin_bit_cast(Any16, o);
+    uint32_t x0 = pack2<T>(v[R * 4], v[R * 4 + 1]), x1 = pack2<T>(v[R * 4 + 2], v[R * 4 + 3]);
+    uint32_t y0 = pack2<T>(v[8 + R * 4], v[8 + R * 4 + 1]), y1 = pack2<T>(v[8 + R * 4 + 2], v[8 + R * 4 + 3]);
+    exchange<32>(x0, y0);
+    exchange<32>(x1, y1);
+    const Any16 o = {{x0, x1, y0, y1}};
+    if (left >= 8) *reinterpret_cast<Any16 *>((T *)to + at) = o;
+    else
+#pragma unroll
+        for (int e = 0; e < 7; e++)
+            if (e < left) ((uint16_t *)to)[at + e] = (uint16_t)(o.w[e / 2] >> (16 * (e & 1)));
+}
+// the same places of a matrix that is read: eight columns of row R as they lie in memory, and (exchanged back) as the turned block has them
+__device__ __forceinline__ Any16 load_joined(const void *from, uint64_t at, int left)
+{
+    Any16 r = {{0, 0, 0, 0}};
+    if (left >= 8) r = *reinterpret_cast<const Any16 *>((const uint16_t *)from + at);
+    else
+#pragma unroll
+        for (int e = 0; e < 7; e++)
+            if (e < left) r.w[e / 2] |= (uint32_t)((const uint16_t *)from)[at + e] << (16 * (e & 1));
+    return r;
+}
+template <class T> __device__ __forceinline__ void part_joined(const Any16 &r, f32x4 (&c)[2])      // c[u]: columns of the u-th 16
+{
+    uint32_t x0 = r.w[0], x1 = r.w[1], y0 = r.w[2], y1 = r.w[3];
+    exchange<32>(x0, y0);
+    exchange<32>(x1, y1);
+    struct Q { T v[4]; };
+    struct W { uint32_t a, b; };
+    const Q p = __builtin_bit_cast(Q, (W{x0, x1})), q = __builtin_bit_cast(Q, (W{y0, y1}));
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        c[0][e] = (float)p.v[e];
+        c[1][e] = (float)q.v[e];
+    }
 }
 
-template <class T, int P, int ACT, bool Y32, bool RES>
-__device__ __forceinline__ void epilogue_plain(const Linear &g, const BigItem &c, const f32x16 (&acc)[4][2], int wm, int wn, int rot)
+// 32 x 32 results at a time, straight from the accumulators.  What is read is asked for one block ahead.  Results in 32 bits (Y32) or
+// the operands' type; a residual in 32 bits (RES32) or the operands' type (RES16).
+template <class T, int P, int ACT, bool Y32, int RES>
+__device__ __forceinline__ void epilogue(const Linear &g, const BigItem &c, const f32x16 (&acc)[4][2], int wm, int wn, int rot)
 {
-    constexpr int own = own_type<T>();
-    const int lane = threadIdx.x & 63, h = lane >> 5;
-    const uint32_t m0 = c.m0 + wm + (lane & 31), n0 = c.n0 + wn, N = (uint32_t)g.N, M = (uint32_t)g.M;
-    const uint32_t nq = n0 + h * 4, nj = n0 + h * 8;           // this lane's columns of a group, and of two groups joined
-    constexpr bool with_res = RES, with_pre = P == GIN && ACT;      // known here: a load that might not be used would be waited for in the loop
-    RawQuad res[2][4], pre[2][4];
+    const int lane = threadIdx.x & 63, h = lane >> 5, b4 = (lane >> 4) & 1;
+    const uint32_t m0 = c.m0 + wm + (lane & 15), n0 = c.n0 + wn, N = (uint32_t)g.N, M = (uint32_t)g.M;
+    const uint32_t nq = n0 + b4 * 8 + h * 4, nj = n0 + h * 16 + b4 * 8;       // this lane's columns: four of each 16, and eight of 32
+    constexpr bool with_pre = P == GIN && ACT;                 // known here: a load that might not be used would be waited for in the loop
+    f32x4 res32[RES == RES32 ? 2 : 1][2][2];
+    Any16 res16[2][2], pre[2][2];
     auto ask = [&](int t) __attribute__((always_inline)) {
-        const uint32_t m = m0 + (((t >> 1) + rot) & 3) * 32;
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            const uint32_t n = nq + (t & 1) * 32 + q * 8;
-            const int w = m < M && n < N ? 4 : 0;
-            if (with_res) res[t & 1][q] = load_raw(g.res, g.res_type, m * g.ldr + n, w);
-            if (with_pre) pre[t & 1][q] = load_raw(g.pre_in, own, m * g.ldp + n, w);
+        for (int R = 0; R < 2; R++) {
+            const uint32_t m = m0 + (((t >> 1) + rot) & 3) * 32 + R * 16, n = nj + (t & 1) * 32;
+            if constexpr (RES == RES32)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const uint32_t at = nq + (t & 1) * 32 + u * 16;
+                    res32[t & 1][R][u] = load4_typed(g.res, OPAL_F32, m * g.ldr + at, m < M ? (int)(N - at) : 0);
+                }
+            if (RES == RES16) res16[t & 1][R] = load_joined(g.res, m * g.ldr + n, m < M ? (int)(N - n) : 0);
+            if (with_pre) pre[t & 1][R] = load_joined(g.pre_in, m * g.ldp + n, m < M ? (int)(N - n) : 0);
         }
     };
-    if (with_res || with_pre) ask(0);
-    f32x4 bias[2][4] = {};
+    if (RES || with_pre) ask(0);
+    f32x4 bias[2][2] = {};
     if (P == FWD && g.bias)
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int q = 0; q < 4; q++)
-                if (nq + j * 32 + q * 8 < N) bias[j][q] = load4(g.bias + nq + j * 32 + q * 8);
+            for (int u = 0; u < 2; u++)
+                bias[j][u] = load4_typed(g.bias, OPAL_F32, nq + j * 32 + u * 16, (int)(N - (nq + j * 32 + u * 16)));
 #pragma unroll
     for (int t = 0; t < 8; t++) {
-        const uint32_t m = m0 + (((t >> 1) + rot) & 3) * 32;
         f32x16 v = acc[t >> 1][t & 1];
-        if ((with_res || with_pre) && t < 7) ask(t + 1);
+        if ((RES || with_pre) && t < 7) ask(t + 1);
+        turn16(v);
         if (P == FWD) {
 #pragma unroll
-            for (int q = 0; q < 4; q++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[q * 4 + e] += bias[t & 1][q][e];
+            for (int e = 0; e < 16; e++) v[e] += bias[t & 1][e >> 3][e & 3];
         }
+        const uint32_t m = m0 + (((t >> 1) + rot) & 3) * 32, n = nj + (t & 1) * 32;
         if (P == FWD && g.pre_out) {
 #pragma unroll
-            for (int qq = 0; qq < 2; qq++) {
-                const uint32_t n = nj + (t & 1) * 32 + qq * 16;
-                store_joined<T>(g.pre_out, m * g.ldp + n, m < M && n < N, v, qq);
-            }
+            for (int R = 0; R < 2; R++) store_joined<T>(g.pre_out, (m + R * 16) * g.ldp + n, m + R * 16 < M ? (int)(N - n) : 0, v, R);
         }
         if (P == FWD && ACT) {
 #pragma unroll
             for (int e = 0; e < 16; e++) v[e] = act_value(v[e], ACT);
         }
-        if (with_pre) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const f32x4 z = decode(pre[t & 1][q], own);
+        for (int R = 0; R < 2; R++) {
+            if (with_pre) {
+                f32x4 z[2];
+                part_joined<T>(pre[t & 1][R], z);
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[q * 4 + e] *= act_slope(z[e], ACT);
+                for (int e = 0; e < 8; e++) v[(e >> 2) * 8 + R * 4 + (e & 3)] *= act_slope(z[e >> 2][e & 3], ACT);
             }
-        }
-        if (with_res) {
+            if (RES) {
+                f32x4 r[2];
+                if constexpr (RES == RES32) {
+                    r[0] = res32[t & 1][R][0];
+                    r[1] = res32[t & 1][R][1];
+                } else part_joined<T>(res16[t & 1][R], r);
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const f32x4 r = decode(res[t & 1][q], g.res_type);
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[q * 4 + e] += r[e];
+                for (int e = 0; e < 8; e++) v[(e >> 2) * 8 + R * 4 + (e & 3)] += r[e >> 2][e & 3];
             }
-        }
-        if constexpr (Y32) {
+            if constexpr (Y32) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const uint32_t n = nq + (t & 1) * 32 + q * 8;
-                if (m < M && n < N) store4((float *)g.y + c.split * g.y_split + m * g.ldy + n, f32x4{v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]});
-            }
-        } else {
-#pragma unroll
-            for (int qq = 0; qq < 2; qq++) {
-                const uint32_t n = nj + (t & 1) * 32 + qq * 16;
-                store_joined<T>(g.y, m * g.ldy + n, m < M && n < N, v, qq);
-            }
+                for (int u = 0; u < 2; u++) {
+                    const uint32_t at = nq + (t & 1) * 32 + u * 16;
+                    store4_typed(g.y, OPAL_F32, c.split * g.y_split + (m + R * 16) * g.ldy + at, m + R * 16 < M ? (int)(N - at) : 0,
+                                 f32x4{v[u * 8 + R * 4], v[u * 8 + R * 4 + 1], v[u * 8 + R * 4 + 2], v[u * 8 + R * 4 + 3]});
+                }
+            } else store_joined<T>(g.y, (m + R * 16) * g.ldy + n, m + R * 16 < M ? (int)(N - n) : 0, v, R);
         }
     }
 }
@@ -470,12 +428,12 @@ __device__ __forceinline__ void big_step(Feed<P> &feed, f32x16 (&acc)[4][2], cha
     }
 }
 
-template <class T, int P, int ACT, bool Y32, bool RES> __global__ __launch_bounds__(BIG_THREADS, 1) void linear_big_kernel(const Linear)
+template <class T, int P, int ACT, bool Y32, int RES> __global__ __launch_bounds__(BIG_THREADS, 1) void linear_big_kernel(const Linear)
 {
     using RA = Ring<P, true>;
     using RB = Ring<P, false>;
     static_assert(RA::N == RB::N && RA::PARTS <= 2, "");
-    __shared__ __attribute__((aligned(128))) char lds[RA::N * RA::BYTES + RB::N * RB::BYTES + 8 * BIG_TURN];
+    __shared__ __attribute__((aligned(128))) char lds[RA::N * RA::BYTES + RB::N * RB::BYTES];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave >> 2;
     Feed<P> feed;
     feed.init(wave);
@@ -521,16 +479,12 @@ template <class T, int P, int ACT, bool Y32, bool RES> __global__ __launch_bound
         landed = ahead - 1;
         const Linear &g = reload();
         const BigItem c = big_item<P>(g, ci);
-        constexpr int own = own_type<T>();
         if (P == GWT && sum_rows) {
             colsum += __shfl_xor(colsum, 32, WAVE);            // the two halves of each 16 k
             const uint32_t m = c.m0 + half * 128 + (wave & 3) * 32 + (threadIdx.x & 31);
             if ((threadIdx.x & 32) == 0 && m < g.M) g.colsum[c.split * g.M + m] = colsum;
         }
-        const bool plain = (g.N - c.n0 >= BIG || g.N % 8 == 0) && g.y_type == (Y32 ? OPAL_F32 : own) && (!RES || g.res_type == OPAL_F32 || g.res_type == own);
-        if (plain) epilogue_plain<T, P, ACT, Y32, RES>(g, c, acc, half * 128, (wave & 3) * 64, P == GWT ? wave & 3 : 0);
-        else epilogue_any<T, P, ACT>(g, c, acc, reinterpret_cast<float *>(lds + RA::N * RA::BYTES + RB::N * RB::BYTES + wave * BIG_TURN), half * 128, (wave & 3) * 64,
-                                         P == GWT ? wave & 3 : 0);
+        epilogue<T, P, ACT, Y32, RES>(g, c, acc, half * 128, (wave & 3) * 64, P == GWT ? wave & 3 : 0);
         ci += g.blocks;
         if (ci >= g.items) break;
         if (half) asm volatile("s_barrier" ::: "memory");
@@ -542,18 +496,18 @@ template <class T, int P, int ACT, bool Y32, bool RES> __global__ __launch_bound
 template <class T> hipError_t launch_big(const Linear &g, int product, hipStream_t stream)
 {
 #define OPAL_BIG(P, ACT, Y32, RES)                                                                                          \
-    if (product == P && (P == GWT || (g.act == ACT && (g.y_type == OPAL_F32) == Y32 && (g.res != nullptr) == RES))) {        \
+    if (product == P && (P == GWT || (g.act == ACT && (g.y_type == OPAL_F32) == Y32 && (!g.res ? 0 : g.res_type == OPAL_F32 ? RES32 : RES16) == RES))) {        \
         hipLaunchKernelGGL((linear_big_kernel<T, P, ACT, Y32, RES>), dim3(g.blocks), dim3(BIG_THREADS), 0, stream, g);       \
         return hipGetLastError();                                                                                           \
     }
 #define OPAL_BIGS2(P, Y32, RES) \
     OPAL_BIG(P, ACT_NONE, Y32, RES) OPAL_BIG(P, ACT_RELU, Y32, RES) OPAL_BIG(P, ACT_SILU, Y32, RES) OPAL_BIG(P, ACT_GELU, Y32, RES)
-#define OPAL_BIGS(P, Y32) OPAL_BIGS2(P, Y32, false) OPAL_BIGS2(P, Y32, true)
+#define OPAL_BIGS(P, Y32) OPAL_BIGS2(P, Y32, 0) OPAL_BIGS2(P, Y32, RES16) OPAL_BIGS2(P, Y32, RES32)
     OPAL_BIGS(FWD, false)
     OPAL_BIGS(FWD, true)
     OPAL_BIGS(GIN, false)
     OPAL_BIGS(GIN, true)
-    OPAL_BIG(GWT, ACT_NONE, true, false)
+    OPAL_BIG(GWT, ACT_NONE, true, 0)
 #undef OPAL_BIGS
 #undef OPAL_BIGS2
 #undef OPAL_BIG

@@ -375,7 +375,7 @@ class Engine:
 
     # ------------------------------------------------------------------ score head (operators behind the per-class scores)
     # Matrices are torch tensors [n, cols] on the engine's GPU, float32 / float16 / bfloat16, whose last stride is 1 and whose row
-    # stride is at least cols (a view into wider rows is fine); new ones get rows of a multiple of 16 bytes.  The work runs on the
+    # stride is at least cols (a view into wider rows is fine); new ones get rows of a multiple of 16 or 128 bytes.  The work runs on the
     # engine's stream; when torch's current stream is another one, the two are ordered before and after the call.
     # (What every call does is kept short: a call for one read is as long as its host side.)
     def _matrix(self, x, name, rows=None, cols=None, dtype=None):
@@ -413,11 +413,14 @@ class Engine:
         return x.data_ptr()
 
     def _new(self, n, cols, dtype):
-        """An uninitialised matrix whose rows begin on 16 bytes: (tensor, address, element type, row stride)."""
+        """An uninitialised matrix: (tensor, address, element type, row stride).  Rows begin on 16 bytes, which the kernels' wide reads need;
+        rows of 1 KB or more on 128, so that a tile's part of a row is whole cache lines (60 001 x 1563 float32 logits: 273 -> 252 us)."""
         kind = self._types.get(dtype)
         if kind is None:
             raise ValueError("%s: must be float32, float16 or bfloat16" % dtype)
-        ld = (cols + 3) & ~3 if kind == _lib.OPAL_F32 else (cols + 7) & ~7
+        each = 4 if kind == _lib.OPAL_F32 else 2
+        step = (128 if cols * each >= 1024 else 16) // each
+        ld = (cols + step - 1) & -step
         t = self.torch
         y = t.empty((n, cols), dtype=dtype, device=self.device) if ld == cols else t.empty_strided((n, cols), (ld, 1), dtype=dtype, device=self.device)
         return y, y.data_ptr(), kind, ld
