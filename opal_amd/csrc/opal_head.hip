@@ -686,7 +686,7 @@ static hipError_t launch(const Linear &g, int type, int product, int tile, bool 
     return launch_linear<bf16_t>(g, product, tile, dma, st);
 }
 
-constexpr int TILE_M[] = {64, 128, 256, 0, 128}, TILE_N[] = {64, 128, 256, 0, 256};
+constexpr int TILE_M[] = {64, 128, 256, 0, 128, 32}, TILE_N[] = {64, 128, 256, 0, 256, 32};
 
 static uint64_t tiles_of(uint64_t M, uint64_t N, int tile) { return ((M + TILE_M[tile] - 1) / TILE_M[tile]) * ((N + TILE_N[tile] - 1) / TILE_N[tile]); }
 
@@ -844,11 +844,15 @@ extern "C" int opal_linear_grad_input(opal_ctx *ctx, const void *d_dy, uint64_t 
 }
 
 // Splits of the sum over the rows, none empty.  256 x 256 tiles: as many as give the 256 CUs a tile each, of at least 16 steps.
-// Smaller ones: two blocks per CU, of at least four steps.  The choice does not look at the operands' alignment, so that the workspace
+// Smaller ones: two blocks per CU, of at least four steps.  Few rows, while 32 x 32 tiles find a CU each, are one block's for all of the
+// sum, without splits to add up: 1999 x 355 x 63 (rows, in, out) 5.3 us against 4.8 and 4.6 for the splits' sum; 4096 x 355 x 128 8.8 against
+// 10.2 + 4.6, 8192 x 355 x 128 26 against 10.6 + 4.6; 32-bit types, whose operands are loads of one column, 1024 x 512 x 512 10.0 against 13.6 +
+// 4.6, 1024 x 384 x 64 9.8 against 5.5 + 4.6, 1999 x 355 x 63 15.7 against 5.9 + 4.6.  The choice does not look at the operands' alignment, so that the workspace
 // does not depend on it; unaligned operands take 128 x 128 tiles in the same splits.
 struct Splits { int tile; uint64_t splits, rows; };
 static Splits weight_splits(uint64_t n, uint32_t in, uint32_t out, int type)
 {
+    if (n <= (type == OPAL_F32 ? 1024 : 4096) && tiles_of(out, in, 5) <= 256) return {5, 1, n};
     const uint64_t step = STEP_BYTES / type_bytes(type);
     const uint64_t steps = std::max<uint64_t>((n + step - 1) / step, 1);
     const uint64_t big = tiles_of(out, in, 2);

@@ -529,8 +529,143 @@ template <class T, int P, int TM> __global__ __launch_bounds__(FEW_WAVES * WAVE)
     finish_quad<T, P>(g, v, m, n, ncol, P == FWD && g.bias ? load4_typed(g.bias, OPAL_F32, n, ncol) : f32x4{0.f, 0.f, 0.f, 0.f}, 0);
 }
 
+// GWT of few rows: a block takes 32 x 32 results over all rows, which its sixteen waves share between them, and adds up in LDS: one launch
+// and no workspace, where splits would need a second launch to add them up.  Operands come straight from memory, all of a wave's
+// loads for 64 rows (32 of 32-bit types) at once.  16 bits: a lane loads two neighbouring columns of eight rows; its even ones are one operand of
+// v_mfma_f32_16x16x32, its odd ones another.
+constexpr int FEWW_WAVES = 16, FEWW_LD = 33;
+
+template <class T> struct FewCols {            // a lane's loads of one operand
+    static constexpr bool W16 = sizeof(T) == 2;
+    static constexpr int ROWS = W16 ? 8 : 1, PER = W16 ? 32 : 4, NV = W16 ? 8 : 2;      // rows of a lane and of a wave, registers
+    const char *p;
+    uint64_t ld;                               // (the same for all lanes, as p)
+    uint32_t off, more;                        // more: 32 bits: the other 16 columns are the next ones, or these again
+    int row;                                   // this lane's first row
+    bool edge;                                 // 16 bits: the second column is behind the matrix's edge
+    // columns c0 .. c0 + 31 of `cols`; lanes behind the edge read its last ones (whose results nobody writes)
+    __device__ __forceinline__ void init(const char *base, uint64_t stride, uint32_t c0, uint32_t cols, int lane)
+    {
+        uint32_t c = c0 + (W16 ? 2 : 1) * (lane & 15);
+        if (c >= cols) c = W16 ? (cols - 1) & ~1u : cols - 1;
+        ld = stride * sizeof(T);
+        p = base;
+        row = (lane >> 4) * ROWS;
+        off = (uint32_t)row * (uint32_t)ld + c * sizeof(T);          // less than 2^28: 24 rows of 2^22 bytes
+        more = c + 16 < cols ? 64 : 0;
+        edge = W16 && c + 1 == cols;
+    }
+    // This lane's rows of those from k on; CUT: those from `end` on as zeros, and nothing behind the edge (which, in all rows but the
+    // matrix's last, is the next element in memory: read with its neighbour, used by no result).
+    template <bool CUT> __device__ __forceinline__ void load(uint64_t k, uint64_t end, uint32_t (&v)[NV]) const
+    {
+        struct __attribute__((packed, aligned(2))) Any { uint32_t w; };
+#pragma unroll
+        for (int e = 0; e < NV; e++) {
+            const uint64_t r = k + (W16 ? e : 0);
+            v[e] = 0;
+            if (CUT && r + row >= end) continue;
+            const char *q = p + r * ld + (off + (W16 ? 0 : e * more));
+            if (CUT && edge) v[e] = *reinterpret_cast<const uint16_t *>(q);
+            else v[e] = reinterpret_cast<const Any *>(q)->w;
+        }
+    }
+};
+
+template <class T> __global__ __launch_bounds__(FEWW_WAVES * WAVE) void linear_few_weight_kernel(const Linear g)
+{
+    using C = FewCols<T>;
+    constexpr bool W16 = C::W16;
+    constexpr int NV = C::NV, U = W16 ? 2 : 8;
+    __shared__ float red[FEWW_WAVES][32 * FEWW_LD];
+    __shared__ float sums[FEWW_WAVES * 4][32];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c16 = lane & 15;
+    const uint32_t n0 = (blockIdx.x % g.tn) * 32, m0 = (blockIdx.x / g.tn) * 32;
+    C a, b;
+    a.init(g.a, g.lda, m0, (uint32_t)g.M, lane);
+    b.init(g.b, g.ldb, n0, (uint32_t)g.N, lane);
+    const bool sum_rows = n0 == 0 && g.colsum;
+    f32x4 acc[2][2];                           // [n][m]: even and odd columns (16 bits), the first and the second sixteen
+#pragma unroll
+    for (int i = 0; i < 2; i++) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float cs[2] = {0.f, 0.f};
+    auto use = [&](const uint32_t (&va)[NV], const uint32_t (&vb)[NV]) __attribute__((always_inline)) {
+        u32x4 fa[2], fb[2];
+        if constexpr (W16) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                fa[0][i] = __builtin_amdgcn_perm(va[2 * i + 1], va[2 * i], 0x05040100);
+                fa[1][i] = __builtin_amdgcn_perm(va[2 * i + 1], va[2 * i], 0x07060302);
+                fb[0][i] = __builtin_amdgcn_perm(vb[2 * i + 1], vb[2 * i], 0x05040100);
+                fb[1][i] = __builtin_amdgcn_perm(vb[2 * i + 1], vb[2 * i], 0x07060302);
+            }
+            if (sum_rows) {
+                cs[0] += sum8<T>(__builtin_bit_cast(s16x8, fa[0]));
+                cs[1] += sum8<T>(__builtin_bit_cast(s16x8, fa[1]));
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) acc[i][j] = mfma_few<T>(fb[i], fa[j], acc[i][j]);
+        } else {
+            const float x0 = __builtin_bit_cast(float, va[0]), x1 = __builtin_bit_cast(float, va[1]), y0 = __builtin_bit_cast(float, vb[0]), y1 = __builtin_bit_cast(float, vb[1]);
+            if (sum_rows) {
+                cs[0] += x0;
+                cs[1] += x1;
+            }
+#ifdef __HIP_DEVICE_COMPILE__
+            acc[0][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(y0, x0, acc[0][0], 0, 0, 0);
+            acc[0][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(y0, x1, acc[0][1], 0, 0, 0);
+            acc[1][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(y1, x0, acc[1][0], 0, 0, 0);
+            acc[1][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(y1, x1, acc[1][1], 0, 0, 0);
+#endif
+        }
+    };
+    uint64_t k = (uint64_t)wave * (U * C::PER);
+    for (; k + U * C::PER < g.K; k += (uint64_t)FEWW_WAVES * U * C::PER) {
+        uint32_t va[U][NV], vb[U][NV];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            a.template load<false>(k + u * C::PER, 0, va[u]);
+            b.template load<false>(k + u * C::PER, 0, vb[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) use(va[u], vb[u]);
+    }
+    for (uint64_t end = k + U * C::PER < g.K ? k + U * C::PER : g.K; k < end; k += C::PER) {      // the rows up to the last one, one wave's
+        uint32_t va[NV], vb[NV];
+        a.template load<true>(k, g.K, va);
+        b.template load<true>(k, g.K, vb);
+        use(va, vb);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int n = (lane >> 4) * 4 + r;
+                red[wave][(W16 ? 2 * c16 + j : j * 16 + c16) * FEWW_LD + (W16 ? 2 * n + i : i * 16 + n)] = acc[i][j][r];
+            }
+    if (sum_rows)
+#pragma unroll
+        for (int j = 0; j < 2; j++) sums[wave * 4 + (lane >> 4)][W16 ? 2 * c16 + j : j * 16 + c16] = cs[j];
+    __syncthreads();
+    const uint32_t r = threadIdx.x >> 5, c = threadIdx.x & 31;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < FEWW_WAVES; w++) v += red[w][r * FEWW_LD + c];
+    if (m0 + r < g.M && n0 + c < g.N) ((float *)g.y)[(uint64_t)(m0 + r) * g.ldy + n0 + c] = v;
+    if (sum_rows && threadIdx.x < 32 && m0 + c < g.M) {
+        v = 0.f;
+#pragma unroll 8
+        for (int w = 0; w < FEWW_WAVES * 4; w++) v += sums[w][c];
+        g.colsum[m0 + c] = v;
+    }
+}
+
 // The launch of one product in one element type (opal_linear_{f32,f16,bf16}.hip); tile: 0 = 64 x 64, 1 = 128 x 128, 2 = 256 x 256
-// (16-bit types on the aligned path only), 3 = few rows (g.few x 16), 4 = 128 x 256 (FWD, as 2).
+// (16-bit types on the aligned path only), 3 = few rows (g.few x 16), 4 = 128 x 256 (FWD, as 2), 5 = 32 x 32 over all rows (GWT).
 template <class T> hipError_t launch_linear(const Linear &g, int product, int tile, bool dma, hipStream_t stream);
 
 #define OPAL_LINEAR_CASE(T, P, TILE, BM, BN, WM, WN, D)                                                                              \
@@ -541,6 +676,11 @@ template <class T> hipError_t launch_linear(const Linear &g, int product, int ti
 #define OPAL_LINEAR_FEW(T, P, TM)                                                                                                   \
     if (product == P && tile == 3 && g.few == TM) {                                                                                  \
         hipLaunchKernelGGL((linear_few_kernel<T, P, TM>), dim3(g.tm * g.tn), dim3(FEW_WAVES * WAVE), 0, stream, g);                   \
+        return hipGetLastError();                                                                                                    \
+    }
+#define OPAL_LINEAR_FEW_WEIGHT(T)                                                                                                   \
+    if (product == GWT && tile == 5) {                                                                                               \
+        hipLaunchKernelGGL((linear_few_weight_kernel<T>), dim3(g.tm * g.tn), dim3(FEWW_WAVES * WAVE), 0, stream, g);                  \
         return hipGetLastError();                                                                                                    \
     }
 #define OPAL_LINEAR_CASES(T, P)                       \

@@ -6,6 +6,7 @@ template <> hipError_t launch_linear<bf16_t>(const Linear &g, int product, int t
 {
     if (tile == 4 && dma && product == FWD) return launch_pair<bf16_t>(g, stream);
     if (tile == 2 && dma) return launch_big<bf16_t>(g, product, stream);
+    OPAL_LINEAR_FEW_WEIGHT(bf16_t)
     OPAL_LINEAR_CASES(bf16_t, FWD)
     OPAL_LINEAR_CASES(bf16_t, GIN)
     OPAL_LINEAR_CASES(bf16_t, GWT)

@@ -6,6 +6,7 @@ template <> hipError_t launch_linear<f16_t>(const Linear &g, int product, int ti
 {
     if (tile == 4 && dma && product == FWD) return launch_pair<f16_t>(g, stream);
     if (tile == 2 && dma) return launch_big<f16_t>(g, product, stream);
+    OPAL_LINEAR_FEW_WEIGHT(f16_t)
     OPAL_LINEAR_CASES(f16_t, FWD)
     OPAL_LINEAR_CASES(f16_t, GIN)
     OPAL_LINEAR_CASES(f16_t, GWT)

@@ -214,6 +214,7 @@ class Engine:
         self._lib = lib()
         # the handle of a device's current stream: the short way where torch has it (0.1 us against 1.9)
         self._current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+        self._index, self._f32 = self.device.index, torch.float32
         self._types = {torch.float32: _lib.OPAL_F32, torch.float16: _lib.OPAL_F16, torch.bfloat16: _lib.OPAL_BF16}
         h = C.c_void_p()
         check(lib().opal_ctx_create(device, stream, C.byref(h)))
@@ -384,7 +385,7 @@ class Engine:
             n, c = x.shape
             ld, one = x.stride()
             kind = self._types[x.dtype]
-            here = x.get_device() == self.device.index
+            here = x.get_device() == self._index
         except (AttributeError, KeyError, ValueError, TypeError):
             raise ValueError("%s must be a matrix (2-d tensor) of float32, float16 or bfloat16 on %s" % (name, self.device)) from None
         if not here:
@@ -403,13 +404,13 @@ class Engine:
         """Address of a vector argument, checked; None for None."""
         if x is None:
             return None
-        dtype = dtype or self.torch.float32
         try:
-            good = x.dtype == dtype and x.shape == (n,) and (n <= 1 or x.stride(0) == 1) and x.get_device() == self.device.index
-        except AttributeError:
+            (m,) = x.shape
+            good = m == n and x.dtype is (dtype or self._f32) and x.is_contiguous() and x.get_device() == self._index
+        except (AttributeError, TypeError, ValueError):
             good = False
         if not good:
-            raise ValueError("%s must be a contiguous %s vector of %d on %s" % (name, dtype, n, self.device))
+            raise ValueError("%s must be a contiguous %s vector of %d on %s" % (name, dtype or self._f32, n, self.device))
         return x.data_ptr()
 
     def _new(self, n, cols, dtype):
@@ -421,13 +422,12 @@ class Engine:
         each = 4 if kind == _lib.OPAL_F32 else 2
         step = (128 if cols * each >= 1024 else 16) // each
         ld = (cols + step - 1) & -step
-        t = self.torch
-        y = t.empty((n, cols), dtype=dtype, device=self.device) if ld == cols else t.empty_strided((n, cols), (ld, 1), dtype=dtype, device=self.device)
+        y = self.torch.empty_strided((n, cols), (ld, 1), dtype=dtype, device=self.device)
         return y, y.data_ptr(), kind, ld
 
     def _run(self, call, tensors, *args):
         """One C call on the engine's stream, ordered with torch's current stream when that is another one."""
-        if self._current(self.device.index) == self._stream:
+        if self._current(self._index) == self._stream:
             rc = call(self._h, *args)
             if rc:
                 check(rc, self._h)

@@ -75,7 +75,7 @@ def slope64(v, a):
 
 
 # every product: sizes around the tiles' and steps' edges, one row, odd sizes, strides that break the 16-byte alignment
-SHAPES = [(1, 1, 1), (1, 356, 64), (3, 7, 5), (64, 64, 64), (65, 63, 66), (130, 129, 127), (17, 355, 100), (200, 1563, 33), (129, 40, 1564), (700, 72, 260), (2049, 130, 129)]
+SHAPES = [(1, 1, 1), (1, 356, 64), (3, 7, 5), (64, 64, 64), (65, 63, 66), (130, 129, 127), (17, 355, 100), (200, 1563, 33), (129, 40, 1564), (700, 72, 260), (2049, 130, 129), (4500, 130, 66), (5003, 33, 65)]
 
 
 @pytest.mark.gpu
