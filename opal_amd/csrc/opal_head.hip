@@ -844,7 +844,8 @@ extern "C" int opal_linear_grad_input(opal_ctx *ctx, const void *d_dy, uint64_t 
 }
 
 // Splits of the sum over the rows, none empty.  256 x 256 tiles: as many as give the 256 CUs a tile each, of at least 16 steps.
-// Smaller ones: two blocks per CU, of at least four steps.  Few rows, while 32 x 32 tiles find a CU each, are one block's for all of the
+// Smaller ones: two blocks per CU, of at least four steps; 128 x 128 from twelve on: 20 000 x 512 x 512 (16 tiles) 16.3 us against 22.3 with 64 x
+// 64, 6000 x 1564 x 512 (52) 16.8 against 22.0; below it 8192 x 512 x 256 (8) 9.2 against 7.1, 20 000 x 355 x 128 (3) 12.1 against 7.5.  Few rows, while 32 x 32 tiles find a CU each, are one block's for all of the
 // sum, without splits to add up: 1999 x 355 x 63 (rows, in, out) 5.3 us against 4.8 and 4.6 for the splits' sum; 4096 x 355 x 128 8.8 against
 // 10.2 + 4.6, 8192 x 355 x 128 26 against 10.6 + 4.6; 32-bit types, whose operands are loads of one column, 1024 x 512 x 512 10.0 against 13.6 +
 // 4.6, 1024 x 384 x 64 9.8 against 5.5 + 4.6, 1999 x 355 x 63 15.7 against 5.9 + 4.6.  The choice does not look at the operands' alignment, so that the workspace
@@ -857,7 +858,7 @@ static Splits weight_splits(uint64_t n, uint32_t in, uint32_t out, int type)
     const uint64_t steps = std::max<uint64_t>((n + step - 1) / step, 1);
     const uint64_t big = tiles_of(out, in, 2);
     const bool large = type != OPAL_F32 && in > 128 && out > 128 && steps * big >= 16 * 128;
-    const int tile = large ? 2 : in > 64 && out > 64 ? 1 : 0;
+    const int tile = large ? 2 : in > 64 && out > 64 && tiles_of(out, in, 1) >= 12 ? 1 : 0;
     uint64_t s = large ? std::min<uint64_t>(256 / std::min<uint64_t>(big, 256), steps / 16) : std::min<uint64_t>(512 / std::min<uint64_t>(tiles_of(out, in, tile), 512), steps / 4);
     s = std::max<uint64_t>(s, 1);
     const uint64_t per = (steps + s - 1) / s;
@@ -872,37 +873,40 @@ extern "C" uint64_t opal_linear_grad_weight_workspace(uint64_t n, uint32_t in, u
 }
 
 namespace opal_head {
-// The sum of the splits' matrices and of their row sums, in the splits' order: [splits][each] -> dw (rows of `cols`), [splits][out] -> db.
-// Reads what the product has just written; a thread adds up four neighbouring values, eight loads under way.
-__global__ __launch_bounds__(BLOCK) void sum_splits_kernel(const float *part, const float *rows, uint32_t splits, uint64_t each, uint32_t cols, uint32_t out,
-                                                           float *dw, uint64_t ld, float *db)
+// The sum of the splits' matrices and of their row sums: [splits][each] -> dw (rows of `cols`), [splits][out] -> db (or null).  Reads what the
+// product has just written.  A thread adds up four neighbouring values of every G-th split, eight loads under way; G threads, which
+// small matrices need to fill the card, then add up in LDS: always in the same order.
+template <int G> __global__ __launch_bounds__(BLOCK) void sum_splits_kernel(const float *part, const float *rows, uint32_t splits, uint64_t each, uint32_t cols,
+                                                                            uint32_t out, float *dw, uint64_t ld, float *db)
 {
-    const uint64_t quads = (each + 3) / 4, all = quads + (db ? out : 0);
-    for (uint64_t i = (uint64_t)blockIdx.x * BLOCK + threadIdx.x; i < all; i += (uint64_t)gridDim.x * BLOCK) {
-        if (i >= quads) {
-            const uint64_t r = i - quads;
-            float s = rows[r];
-            for (uint32_t p = 1; p < splits; p++) s += rows[(uint64_t)p * out + r];
-            db[r] = s;
-            continue;
-        }
-        const int left = (int)std::min<uint64_t>(each - i * 4, 4);
-        f32x4 s;
-        if (left == 4) {
-            s = load4(part + i * 4);
+    constexpr int QUADS = BLOCK / G;
+    __shared__ f32x4 red[G][QUADS];
+    const int q = threadIdx.x % QUADS, group = threadIdx.x / QUADS;
+    const uint64_t quads = (each + 3) / 4, i = (uint64_t)blockIdx.x * QUADS + q, r = i - quads;
+    const bool row = i >= quads;               // of the row sums, one a thread
+    const int left = !row ? (int)std::min<uint64_t>(each - i * 4, 4) : db && r < out ? 1 : 0;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (left == 4) {
 #pragma unroll 8
-            for (uint32_t p = 1; p < splits; p++) s += load4(part + p * each + i * 4);
-        } else {
-            s = load4_typed(part, OPAL_F32, i * 4, left);
-            for (uint32_t p = 1; p < splits; p++) s += load4_typed(part, OPAL_F32, p * each + i * 4, left);
-        }
-        if (ld == cols) store4_typed(dw, OPAL_F32, i * 4, left, s);
-        else
-            for (int e = 0; e < left; e++) {
-                const uint64_t at = i * 4 + e;
-                dw[at / cols * ld + at % cols] = s[e];
-            }
+        for (uint32_t p = group; p < splits; p += G) s += load4(part + p * each + i * 4);
+    } else if (left) {
+        const float *from = row ? rows + r : part + i * 4;
+        const uint64_t stride = row ? out : each;
+#pragma unroll 8
+        for (uint32_t p = group; p < splits; p += G) s += load4_typed(from, OPAL_F32, p * stride, left);
     }
+    red[group][q] = s;
+    __syncthreads();
+    if (group || !left) return;
+#pragma unroll 8
+    for (int p = 1; p < G; p++) s += red[p][q];
+    if (row) db[r] = s[0];
+    else if (ld == cols) store4_typed(dw, OPAL_F32, i * 4, left, s);
+    else
+        for (int e = 0; e < left; e++) {
+            const uint64_t at = i * 4 + e;
+            dw[at / cols * ld + at % cols] = s[e];
+        }
 }
 }  // namespace opal_head
 
@@ -940,9 +944,15 @@ extern "C" int opal_linear_grad_weight(opal_ctx *ctx, const void *d_dy, uint64_t
     g.colsum = d_dbias ? (part ? rows : d_dbias) : nullptr;
     OPAL_HIP_CHECK(ctx, launch(g, type, GWT, tile, dma, ctx->stream));
     if (part) {
+        // 300 000 x 63 x 64 (512 splits of 4032 values) 138 -> 28 us with 64 threads for each four, 20 000 x 355 x 128 (42 of 45 440) 24.4 -> 15 with 16
         const uint64_t work = (each + 3) / 4 + out;
-        hipLaunchKernelGGL(sum_splits_kernel, dim3((unsigned)std::min<uint64_t>((work + BLOCK - 1) / BLOCK, 8192)), dim3(BLOCK), 0, ctx->stream, part, rows,
-                           (uint32_t)s.splits, each, in, out, d_dw, lddw, d_dbias);
+#define L(G)                                                                                                                              \
+    hipLaunchKernelGGL(sum_splits_kernel<G>, dim3((unsigned)((work + BLOCK / G - 1) / (BLOCK / G))), dim3(BLOCK), 0, ctx->stream, part, rows, \
+                       (uint32_t)s.splits, each, in, out, d_dw, lddw, d_dbias)
+        if (work <= 2048) L(64);
+        else if (work <= 16384) L(16);
+        else L(4);
+#undef L
         OPAL_HIP_CHECK(ctx, hipGetLastError());
     }
     return OPAL_OK;
