@@ -690,31 +690,37 @@ constexpr int TILE_M[] = {64, 128, 256, 0, 128, 32}, TILE_N[] = {64, 128, 256, 0
 
 static uint64_t tiles_of(uint64_t M, uint64_t N, int tile) { return ((M + TILE_M[tile] - 1) / TILE_M[tile]) * ((N + TILE_N[tile] - 1) / TILE_N[tile]); }
 
-// Larger tiles read fewer bytes for the same sums, smaller ones leave fewer CUs idle (us; M x N x K):
-//   128 x 128 instead of 64 x 64 from 1.5 tiles a CU on: 4096 x 512 x 1564 (416 tiles) 14.4 against 15.1, 16384 x 1564 x 512 (512) 34.5 against
-//   49.3; below it 4096 x 1564 x 512 (128) 21.8 against 12.2, 32768 x 356 x 128 (256) 11.5 against 10.7.  32-bit types the same.
+// Larger tiles read fewer bytes for the same sums, smaller ones leave fewer CUs idle and less of a tile outside the matrix (us; rows x N x K):
+//   128 x 128 instead of 64 x 64, 16-bit types, sums of 512 on, from 1.5 tiles a CU on: 16384 x 1564 x 512 34.5 against 49.3, 100 000 x 128 x 1000 49
+//   against 56; below it 4096 x 1564 x 512 (416) 14.4 against 15.1; shorter sums 100 000 x 200 x 200 24.4 against 21.8.  Not where it reaches a
+//   quarter further: 100 000 x 150 x 1000 90 against 83, 100 000 x 64 x 512 26 against 20.  32-bit types, bound by the matrix pipe, never: 50 000 x
+//   512 x 1564 694 against 674, 100 000 x 200 x 150 126 against 82.
 // 16-bit types, aligned:
-//   256 x 256 for sums of 1024 on from one tile a CU on: 32768 x 512 x 1564 (256) 51 against 59 with 128 x 256 and 70 with 128 x 128; below it 16384 x 512
-//   x 1564 (128) 38 against 32 and 35.  For sums of 256 on an input gradient the same (32768 x 512 x 256: 17.5 against 22.3; sums of 128 82 against 73);
-//   a forward product, which has 128 x 256 tiles too, from four on: 250 000 x 355 x 256 (1954) 106 against 110, 100 000 x 1563 x 256 140
-//   against 169; below it 100 000 x 512 x 512 (782) 76 against 70, 32768 x 1564 x 512 (896) 72 against 68.
+//   256 x 256 from one tile a CU on.  Input gradients where it does not reach a quarter further than 128 x 128: 32768 x 512 x 256 17.5 against 22.3, 100 000 x
+//   600 x 64 35 against 44; but 100 000 x 356 x 1000 125 against 113.  Forward products, which have 128 x 256 tiles too, with more than
+//   128 columns and sums of 1024 on (32768 x 512 x 1564 (256) 51 against 59; below it 16384 x 512 x 1564 (128) 38 against 32), or of 256 on from
+//   four tiles a CU on: 250 000 x 355 x 256 (1954) 106 against 110, 100 000 x 1563 x 256 140 against 169; below it 100 000 x 512 x 512 (782) 76
+//   against 70, 32768 x 1564 x 512 (896) 72 against 68.
 //   128 x 256 (forward, more than 128 columns) from 3/4 of a tile a CU on: 250 000 x 355 x 128 66 against 82 with 256 x 256 and 104 with 128 x 128, 4096 x
 //   1564 x 512 (224) 14.1 against 15.5; below it 4099 x 512 x 355 (66) 12.2 against 10.9, 16384 x 200 x 200 (128) 10.9 against 7.7.
 // large: the last two may take it; whole: the first of them too.
-static int pick_tile(int product, uint64_t M, uint64_t N, uint64_t K, int cus, bool large, bool whole)
+static uint64_t reach(uint64_t N, uint64_t tile) { return (N + tile - 1) / tile * tile; }
+static int pick_tile(int product, int type, uint64_t M, uint64_t N, uint64_t K, int cus, bool large, bool whole)
 {
-    const uint64_t c = cus;
-    if (large && whole && K >= 256 && tiles_of(M, N, 2) >= (product == FWD && K < 1024 ? 4 * c : c)) return 2;
+    const uint64_t c = cus, t256 = tiles_of(M, N, 2);
+    if (large && whole && t256 >= c &&
+        (product == FWD ? N > 128 && (K >= 1024 || (K >= 256 && t256 >= 4 * c)) : reach(N, 256) * 4 <= reach(N, 128) * 5)) return 2;
     if (large && product == FWD && N > 128 && tiles_of(M, N, 4) * 4 >= 3 * c) return 4;
-    return tiles_of(M, N, 1) * 2 >= 3 * c ? 1 : 0;
+    return type != OPAL_F32 && K >= 512 && tiles_of(M, N, 1) * 2 >= 3 * c && reach(N, 128) * 4 <= reach(N, 64) * 5 ? 1 : 0;
 }
 
-// The kernel for few rows, while its blocks (64 x 16 results, all of k) find a CU each: 64 x 1564 x 512 in 8.1 us against 10.3 with
-// 64 x 64 tiles, 512 rows (256 blocks) 8.3 against 10.5, 1024 rows 12.6 against 10.7; 2048 x 356 x 100 in 32 bits 7.1 against 11.4.  An
-// input gradient gathers W's columns there one by one: up to 16 rows (9.7 against 10.4 us; 64 rows 13.5 against 10.9).
-static bool few_rows(int product, uint64_t M, uint64_t N, int cus)
+// The kernel for few rows, while its blocks (64 x 16 results, all of k) find a CU each (rows x N x K): 16-bit types 64 x 512 x 1564 8.1 us against 10.3
+// with 64 x 64 tiles, 1024 rows 12.6 against 10.7; an input gradient, which gathers W's columns there one by one, up to 16 rows (9.9
+// against 10.5; 100 rows 13.5 against 10.9).  32-bit types, whose tiles are bound by a wave's chain of MFMAs, both: 512 x 512 x 1564 19
+// against 36, input gradients of 2048 x 100 x 356 6.4 against 10.5; 600 x 1000 x 4000 (630 blocks) 128 against 86.
+static bool few_rows(int product, int type, uint64_t M, uint64_t N, int cus)
 {
-    if (product == GIN && M > 16) return false;
+    if (product == GIN && M > 16 && type != OPAL_F32) return false;
     return ((M + 63) / 64) * ((N + 15) / 16) <= (uint64_t)cus;
 }
 
@@ -744,24 +750,24 @@ static Linear behind(const Linear &g, uint64_t rows, int type)
 
 constexpr uint64_t MOST_TILES = 1u << 24;      // of 256 threads in a launch, which has less than 2^32
 
-static int run_rows(opal_ctx *ctx, const char *who, const Linear &product_of, int type, int product)
+static int run_rows(opal_ctx *ctx, const Linear &product_of, int type, int product)
 {
     Linear g = product_of;
     OnDevice on(ctx->device);
     OPAL_HIP_CHECK(ctx, on.err);
-    constexpr uint64_t SLICE = 1u << 30;       // rows of a launch: up to 2^23 tiles along M
-    if (g.M > SLICE) {
+    // as many rows at a time as the smallest tiles have room for in a launch
+    const uint64_t slice = (MOST_TILES - 1) / ((g.N + TILE_N[0] - 1) / TILE_N[0]) * TILE_M[0] / 256 * 256;
+    if (g.M > slice) {
         Linear q = g;
-        q.M = SLICE;
-        OPAL_TRY(run_rows(ctx, who, q, type, product));
-        g = behind(g, SLICE, type);
+        q.M = slice;
+        OPAL_TRY(run_rows(ctx, q, type, product));
+        return run_rows(ctx, behind(g, slice, type), type, product);
     }
     const bool dma = aligned16(g.a, g.lda, type) && aligned16(g.b, g.ldb, type);
     const int cus = ctx->num_cus;
     // (the two kernels for large products write 32 bits or the operands' type, and read such a residual)
     const bool large = dma && type != OPAL_F32 && (g.y_type == OPAL_F32 || g.y_type == type) && (!g.res || g.res_type == OPAL_F32 || g.res_type == type);
-    int tile = few_rows(product, g.M, g.N, cus) ? 3 : pick_tile(product, g.M, g.N, g.K, cus, large, true);
-    if (tile != 3 && tiles_of(g.M, g.N, tile) >= MOST_TILES) return opal::fail(ctx, OPAL_ERANGE, std::string(who) + ": too many rows times columns for one call");
+    int tile = few_rows(product, type, g.M, g.N, cus) ? 3 : pick_tile(product, type, g.M, g.N, g.K, cus, large, true);
     g.splits = 1;
     g.ksplit = g.K;
     auto run = [&](Linear &q, int t) {
@@ -783,7 +789,7 @@ static int run_rows(opal_ctx *ctx, const char *who, const Linear &product_of, in
         q.M = rows;
         OPAL_HIP_CHECK(ctx, run(q, 2));
         g = behind(g, rows, type);
-        tile = few_rows(product, g.M, g.N, cus) ? 3 : pick_tile(product, g.M, g.N, g.K, cus, large, false);
+        tile = few_rows(product, type, g.M, g.N, cus) ? 3 : pick_tile(product, type, g.M, g.N, g.K, cus, large, false);
     }
     OPAL_HIP_CHECK(ctx, run(g, tile));
     return OPAL_OK;
@@ -813,7 +819,7 @@ extern "C" int opal_linear(opal_ctx *ctx, const void *d_x, uint64_t ldx, const v
     g.res = d_res; g.res_type = res_type; g.ldr = ldr;
     g.y = d_y; g.y_type = y_type; g.ldy = ldy;
     g.pre_out = d_pre; g.ldp = ldp;
-    return run_rows(ctx, who, g, type, FWD);
+    return run_rows(ctx, g, type, FWD);
 }
 
 extern "C" int opal_linear_grad_input(opal_ctx *ctx, const void *d_dy, uint64_t lddy, const void *d_w, uint64_t ldw, int type, const void *d_pre,
@@ -840,7 +846,7 @@ extern "C" int opal_linear_grad_input(opal_ctx *ctx, const void *d_dy, uint64_t 
     g.act = activation; g.pre_in = d_pre; g.ldp = ldp;
     g.res = d_res; g.res_type = res_type; g.ldr = ldr;
     g.y = d_dx; g.y_type = dx_type; g.ldy = lddx;
-    return run_rows(ctx, who, g, type, GIN);
+    return run_rows(ctx, g, type, GIN);
 }
 
 // Splits of the sum over the rows, none empty.  256 x 256 tiles: as many as give the 256 CUs a tile each, of at least 16 steps.

@@ -462,9 +462,8 @@ template <class T, bool KC> __device__ __forceinline__ u32x4 lane_k(const T *p, 
     if (!in || k0 >= K) return v;
     const int left = K - k0 < (uint64_t)EPC ? (int)(K - k0) : EPC;
     if (KC && left == EPC) {
-        struct __attribute__((packed, aligned(sizeof(T)))) Any { uint32_t w[4]; };
-        const Any a = *reinterpret_cast<const Any *>(p + r * ld + k0);
-        return u32x4{a.w[0], a.w[1], a.w[2], a.w[3]};
+        typedef uint32_t Any __attribute__((ext_vector_type(4), aligned(2)));     // (a vector: a struct's 32-bit words would be loaded one by one)
+        return *reinterpret_cast<const Any *>(p + r * ld + k0);
     }
 #pragma unroll
     for (int e = 0; e < EPC; e++)
@@ -683,9 +682,11 @@ template <class T> hipError_t launch_linear(const Linear &g, int product, int ti
         hipLaunchKernelGGL((linear_few_weight_kernel<T>), dim3(g.tm * g.tn), dim3(FEWW_WAVES * WAVE), 0, stream, g);                  \
         return hipGetLastError();                                                                                                    \
     }
-#define OPAL_LINEAR_CASES(T, P)                       \
+#define OPAL_LINEAR_SMALL(T, P)                       \
     OPAL_LINEAR_CASE(T, P, 0, 64, 64, 2, 2, true)     \
-    OPAL_LINEAR_CASE(T, P, 0, 64, 64, 2, 2, false)    \
+    OPAL_LINEAR_CASE(T, P, 0, 64, 64, 2, 2, false)
+#define OPAL_LINEAR_CASES(T, P)                       \
+    OPAL_LINEAR_SMALL(T, P)                           \
     OPAL_LINEAR_CASE(T, P, 1, 128, 128, 2, 2, true)   \
     OPAL_LINEAR_CASE(T, P, 1, 128, 128, 2, 2, false)
 

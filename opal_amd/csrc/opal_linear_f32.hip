@@ -5,8 +5,8 @@ namespace opal_head {
 template <> hipError_t launch_linear<float>(const Linear &g, int product, int tile, bool dma, hipStream_t stream)
 {
     OPAL_LINEAR_FEW_WEIGHT(float)
-    OPAL_LINEAR_CASES(float, FWD)
-    OPAL_LINEAR_CASES(float, GIN)
+    OPAL_LINEAR_SMALL(float, FWD)
+    OPAL_LINEAR_SMALL(float, GIN)
     OPAL_LINEAR_CASES(float, GWT)
     OPAL_LINEAR_FEW(float, FWD, 1)
     OPAL_LINEAR_FEW(float, FWD, 2)
