@@ -74,6 +74,7 @@ __device__ __forceinline__ f32x4 param4(const float *p, int col, int left, float
     return p ? load4_typed(p, OPAL_F32, col, left, none) : f32x4{none, none, none, none};
 }
 
+// Bound by memory: 250 000 x 1564 float32 -> bfloat16 414 us, 5.7 TB/s (a plain conversion of the same matrix: 5.8).
 template <class T, int TPR, int NQ, bool NT> __global__ __launch_bounds__(BLOCK) void norm_kernel(const Norm g)
 {
     __shared__ float red[2 * BLOCK / WAVE];
@@ -113,7 +114,8 @@ template <class T, int TPR, int NQ, bool NT> __global__ __launch_bounds__(BLOCK)
     }
 }
 
-constexpr int LONG = 1024;                // threads on a row that does not fit the registers
+constexpr int LONG = 1024;                // threads on a row that does not fit the registers: read again for each pass, mostly from the caches
+                                          // (20 000 x 20 000 float32 -> bfloat16 1.1 ms, 2.2 TB/s of what it has to read and write)
 
 template <class T> __global__ __launch_bounds__(LONG) void norm_long_kernel(const Norm g)
 {
@@ -155,7 +157,7 @@ constexpr int back_threads(int TPR, int NQ) { return TPR > WAVE ? BLOCK : TPR * 
 
 // Every thread keeps the sums of its own columns over the rows that its team visits; the teams of a block add theirs up in
 // order, and sum_parts_kernel adds the blocks': no atomics, the same bits every time.  The next row is asked for before the
-// present one is worked on.
+// present one is worked on.  Bound by memory: 500 009 x 355 (float32 x and dx, bfloat16 dy) 354 us, 5.0 TB/s, of which the sums' 4.7.
 template <class TX, class TY, int TPR, int NQ> __global__ __launch_bounds__(back_threads(TPR, NQ)) void norm_back_kernel(const NormBack g)
 {
     constexpr int THREADS = back_threads(TPR, NQ), RPB = THREADS / TPR, WAVES = THREADS / WAVE;
@@ -359,6 +361,7 @@ __device__ __forceinline__ int softmax_label(const Softmax &g, uint64_t row, boo
     return bad ? -1 : l - 1;
 }
 
+// Bound by memory: 250 000 x 1564 float32 scores with a bfloat16 gradient 424 us, 5.5 TB/s.
 template <class T, int TPR, int NQ, bool NT> __global__ __launch_bounds__(BLOCK) void softmax_kernel(const Softmax g)
 {
     __shared__ float red[2 * BLOCK / WAVE];
@@ -950,7 +953,7 @@ extern "C" int opal_linear_grad_weight(opal_ctx *ctx, const void *d_dy, uint64_t
     g.colsum = d_dbias ? (part ? rows : d_dbias) : nullptr;
     OPAL_HIP_CHECK(ctx, launch(g, type, GWT, tile, dma, ctx->stream));
     if (part) {
-        // 300 000 x 63 x 64 (512 splits of 4032 values) 138 -> 28 us with 64 threads for each four, 20 000 x 355 x 128 (42 of 45 440) 24.4 -> 15 with 16
+        // 300 000 x 63 x 64 (512 splits of 4032 values) 138 -> 22 us with 64 threads for each four, 20 000 x 355 x 128 (42 of 45 440) 24 -> 14 with 16
         const uint64_t work = (each + 3) / 4 + out;
 #define L(G)                                                                                                                              \
     hipLaunchKernelGGL(sum_splits_kernel<G>, dim3((unsigned)((work + BLOCK / G - 1) / (BLOCK / G))), dim3(BLOCK), 0, ctx->stream, part, rows, \
