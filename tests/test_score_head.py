@@ -204,6 +204,44 @@ def test_large_products_keep_nans_behind_the_edge_out(eng):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("t", [F16, BF16])
+@pytest.mark.parametrize("n,k,m", [(16700, 99, 515), (33000, 1027, 257), (70001, 40, 130), (3000, 33, 63)])
+@pytest.mark.parametrize("wide", [True, False])
+def test_large_products_in_place_and_their_edges(eng, t, n, k, m, wide):
+    """The residual's place may be the result's: the bits are those of a result elsewhere, and what lies between the rows and behind the
+    last one (all NaN) stays what it is."""
+    from opal_amd._lib import check
+    g = torch.Generator(device="cuda").manual_seed(n + k)
+    code, out = {F16: 1, BF16: 2}[t], F32 if wide else t
+
+    def framed(r, c, dt):
+        full = torch.full((r + 2, -(-c // 8) * 8 + 8), float("nan"), device="cuda", dtype=dt)
+        full[:r, :c] = torch.randn(r, c, device="cuda", generator=g)
+        return full, full[:r, :c]
+
+    def untouched(full, r, c):
+        return bool(full[r:].isnan().all()) and bool(full[:, c:].isnan().all())
+    x, w, dy = framed(n, k, t)[1], framed(m, k, t)[1], framed(n, m, t)[1]
+    for a, b, cols, entry in ((x, w, m, "opal_linear"), (dy, w, k, "opal_linear_grad_input")):
+        full, res = framed(n, cols, out)
+        want = eng.linear(a, b, residual=res, out_dtype=out)[0] if entry == "opal_linear" else eng.linear_grad_input(a, b, residual=res, out_dtype=out)
+        oc, ld = {F32: 0, F16: 1, BF16: 2}[out], full.stride(0)
+        if entry == "opal_linear":
+            check(eng._lib.opal_linear(eng._h, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), code, None, 0, full.data_ptr(), oc, ld, n, k, m,
+                                       full.data_ptr(), oc, ld, None, 0), eng._h)
+        else:
+            check(eng._lib.opal_linear_grad_input(eng._h, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), code, None, 0, 0, full.data_ptr(), oc, ld, n, k, m,
+                                                  full.data_ptr(), oc, ld), eng._h)
+        assert torch.isfinite(want).all() and torch.equal(res, want) and untouched(full, n, cols)
+    full, dw = framed(m, k, F32)
+    want, db = eng.linear_grad_weight(dy, x)
+    work = torch.empty(max(eng._lib.opal_linear_grad_weight_workspace(n, k, m, code), 16), dtype=torch.uint8, device="cuda")
+    check(eng._lib.opal_linear_grad_weight(eng._h, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), code, n, k, m, full.data_ptr(), full.stride(0), None,
+                                           work.data_ptr(), work.numel()), eng._h)
+    assert torch.isfinite(want).all() and torch.isfinite(db).all() and torch.equal(dw, want) and untouched(full, m, k)
+
+
+@pytest.mark.gpu
 def test_products_of_no_rows(eng):
     w = torch.randn(5, 7, device="cuda")
     x = torch.empty(0, 7, device="cuda")
