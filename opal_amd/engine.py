@@ -474,9 +474,9 @@ class Engine:
         if want_params:
             dg, db = t.empty(cols, dtype=t.float32, device=self.device), t.empty(cols, dtype=t.float32, device=self.device)
             size = self._lib.opal_layer_norm_backward_workspace(n, cols)
-            work = t.empty(size, dtype=t.uint8, device=self.device)
+            work = t.empty(size, dtype=t.uint8, device=self.device) if size else None
         self._run(self._lib.opal_layer_norm_backward, (dy, x, gamma, mean, rstd, dx, dg, db, work), pd, td, ldd, px, tx, ldx, pg, pm, pr, n, cols, px_out, tx_out,
-                  lddx, dg.data_ptr() if want_params else None, db.data_ptr() if want_params else None, work.data_ptr() if want_params else None, size)
+                  lddx, dg.data_ptr() if want_params else None, db.data_ptr() if want_params else None, work.data_ptr() if size else None, size)
         return dx, dg, db
 
     def linear(self, x, w, bias=None, activation="none", residual=None, out_dtype=None, want_pre=False):
