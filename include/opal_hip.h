@@ -265,7 +265,7 @@ int opal_layer_norm(opal_ctx *ctx, const void *d_x, int x_type, uint64_t ldx, co
 
 /* With h = dy gamma and xh = (x - mean) rstd:  dx = rstd (h - mean(h) - xh mean(h xh)),  dgamma = sum over rows of dy xh,
  * dbeta = sum over rows of dy.  d_dx, d_dgamma, d_dbeta: NULL = not wanted; dx may be dy or x (same type and ld).  d_work:
- * opal_layer_norm_backward_workspace(n, cols) bytes, needed for dgamma / dbeta (OPAL_ERANGE when smaller).           */
+ * opal_layer_norm_backward_workspace(n, cols) bytes (0: none), needed for dgamma / dbeta (OPAL_ERANGE when smaller).  */
 uint64_t opal_layer_norm_backward_workspace(uint64_t n, uint32_t cols);
 int opal_layer_norm_backward(opal_ctx *ctx, const void *d_dy, int dy_type, uint64_t lddy, const void *d_x, int x_type, uint64_t ldx,
                              const float *d_gamma, const float *d_mean, const float *d_rstd, uint64_t n, uint32_t cols, void *d_dx,
@@ -286,7 +286,8 @@ int opal_linear_grad_input(opal_ctx *ctx, const void *d_dy, uint64_t lddy, const
                            uint32_t out, void *d_dx, int dx_type, uint64_t lddx);
 
 /* dw[out, in] = dy[n, out]^T x[n, in] and dbias[out] = sum over rows of dy (NULL = not wanted), in float32.  dy is the gradient
- * before the activation.  d_work: opal_linear_grad_weight_workspace(n, in, out, type) bytes (OPAL_ERANGE when smaller).  */
+ * before the activation.  d_work: opal_linear_grad_weight_workspace(n, in, out, type) bytes (0: none; OPAL_ERANGE when
+ * smaller).                                                                                                        */
 uint64_t opal_linear_grad_weight_workspace(uint64_t n, uint32_t in, uint32_t out, int type);
 int opal_linear_grad_weight(opal_ctx *ctx, const void *d_dy, uint64_t lddy, const void *d_x, uint64_t ldx, int type, uint64_t n, uint32_t in,
                             uint32_t out, float *d_dw, uint64_t lddw, float *d_dbias, void *d_work, uint64_t work_bytes);
