@@ -1,10 +1,11 @@
 // The product kernel for large 16-bit matrices on 16 bytes (opal_linear.h has the products, the operands' layouts and the kernel
 // for everything else): 256 x 256 tiles, eight waves of 128 x 64, one block per CU that stays for all its tiles, steps of 32 k.
 //
-// What bounds it: the matrix pipe and LDS, which are asked for nearly the same time (a step of 32 k: 1024 cycles; 96 KB read at 128 bytes a
-// cycle, 32 KB arriving from memory at 64), so everything else runs beside them.  Sums of the hidden layer's product (250 000 x 512 x 1564):
-// 1613 TFLOP/s without requests, 1146 with them, 1004 with the epilogue (399 us; with bias, GELU and the value before it 470).  Input gradient
-// 100 000 x 512 x 1564 in float16 with GELU 207 us, weight gradient 1564 x 512 of 100 000 rows 185 us and 13 for the splits' sum.
+// What bounds it: a half's turn at the matrix pipe (16 MFMAs, 512 cycles) against the other's reads meanwhile (48 KB of LDS at 125 bytes a
+// cycle and their way), the way of the chunks (32 KB a step; a CU takes 58 bytes a cycle, without loss to its LDS reads), and the
+// clock, which falls under the load.  Sums of the hidden layer's product (250 000 x 512 x 1564) 350 us, 1146 TFLOP/s; with all operands zero 306; with
+// the epilogue 399, with bias, GELU and the value before it 470.  Input gradient 100 000 x 512 x 1564 in float16 with GELU 207 us, weight
+// gradient 1564 x 512 of 100 000 rows 185 us and 12 for the splits' sum.
 //   - Waves 0 .. 3 and 4 .. 7 share the four SIMDs and take turns: while one half multiplies (16 MFMAs, its requests for chunks in
 //     between), the other reads its next fragments, with a barrier at each change; half 1 runs one change behind half 0.
 //   - Chunks come straight into LDS, well ahead and over the ends of tiles.  Half 0 asks for A's, half 1 for B's: vmcnt counts a

@@ -3,9 +3,8 @@
 //
 // With short sums the epilogue, which is bound by memory, is most of a tile; opal_linear_big.h's one block a CU does nothing else
 // meanwhile.  Here what one block waits for (the first chunks of its tile, a barrier, the residual, its stores) the other fills with
-// sums: 250 000 x 355 x 128 in 66 us, 2.6 TB/s and 346 TFLOP/s, against 82.  Long sums are bound by LDS, and narrower tiles ask more of it:
-// 250 000 x 512 x 1564 takes 500 us against 399.  A step of 32 k of both blocks is 1024 cycles of the matrix pipes, 96 KB read at 128
-// bytes a cycle and 48 KB arriving from memory at 64.
+// sums: 250 000 x 355 x 128 in 66 us, 2.6 TB/s and 346 TFLOP/s, against 82.  Long sums are bound by the chunks' way, and narrower tiles ask for
+// more of them: 48 KB for 1024 cycles of the matrix pipes, where a CU takes 58 bytes a cycle; 250 000 x 512 x 1564 takes 500 us against 399.
 //   - A wave reads the next 16 k while it multiplies the present ones; one barrier for each 32 k.
 //   - Chunks come straight into LDS, two steps ahead.  A (from memory): 2 x 64 k, whole 128-byte lines, of which a CU has only so many on
 //     their way; B (W stays in L2): 3 x 32 k.  32 + 48 KB, half of a CU's LDS.
