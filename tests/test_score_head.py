@@ -521,10 +521,10 @@ def test_head_gradients_against_the_formula_and_differences(eng, n, K, H):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("t", [BF16, F32])
-def test_head_step_is_the_same_every_time_and_in_a_graph(eng, t):
+@pytest.mark.parametrize("n,K,H", [(515, 355, 72), (3, 10, 16), (70001, 512, 256)])
+def test_head_step_is_the_same_every_time_and_in_a_graph(eng, t, n, K, H):
     """Equal bits on repetition; captured and replayed with new inputs, with eager work between the replays."""
     import opal_amd
-    n, K, H = 515, 355, 72
     vals = head_inputs(n, K, H, t)
     want = head_step(eng, *[v.cuda() for v in vals], t, 1.0 / n)
     again = head_step(eng, *[v.cuda() for v in vals], t, 1.0 / n)
@@ -555,6 +555,31 @@ def test_head_step_is_the_same_every_time_and_in_a_graph(eng, t):
             assert all(torch.equal(a, b) for a, b in zip(out, ref))
     del graphs
     e.close()
+
+
+@pytest.mark.gpu
+def test_two_engines_at_once(eng):
+    """Two engines on two streams, one of them with large products and one with small ones, side by side: nothing is shared."""
+    import opal_amd
+    sizes = [(70001, 512, 256), (900, 355, 128)]
+    vals = [[v.cuda() for v in head_inputs(n, K, H, BF16, seed=n)] for n, K, H in sizes]
+    want = [head_step(eng, *v, BF16, 1.0 / n) for v, (n, _, _) in zip(vals, sizes)]
+    torch.cuda.synchronize()
+    streams, engines = [torch.cuda.Stream() for _ in sizes], []
+    for st in streams:
+        with torch.cuda.stream(st):
+            engines.append(opal_amd.Engine(0))
+    got = [None, None]
+    for _ in range(4):
+        for j, times in ((0, 1), (1, 8)):
+            with torch.cuda.stream(streams[j]):
+                for _ in range(times):
+                    got[j] = head_step(engines[j], *vals[j], BF16, 1.0 / sizes[j][0])
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    for e in engines:
+        e.close()
 
 
 @pytest.mark.gpu
