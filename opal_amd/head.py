@@ -89,6 +89,24 @@ class ScoreHead:
         """(class int32 [n], 1-based, its probability float32 [n])."""
         return self.engine.softmax_class(self.forward(scores))
 
+    def answers(self, batch, reverse, rows=16384, limit=1 << 30):
+        """predict() of a device batch of fragments.  Always as many rows at a time, the last ones filled up with zeros: another number of
+        rows can choose another product kernel, whose sums have another order, and a fragment's answer must not depend on
+        how many others its piece of the file holds."""
+        from .engine import DeviceBatch
+        e, t = self.engine, self.engine.torch
+        rows = max(1, min(rows, limit // (4 * self.K)))
+        cls, prob = [], []
+        scores = t.empty((rows, self.K), dtype=t.float32, device=e.device)
+        for lo in range(0, batch.n, rows):
+            n = min(batch.n - lo, rows)
+            e.predict(DeviceBatch(batch.data, batch.off[lo:lo + n], batch.len[lo:lo + n], n, batch.nbytes), reverse, want_scores=True, out_scores=scores)
+            scores[n:].zero_()
+            c, p = self.predict(scores)
+            cls.append(c[:n])
+            prob.append(p[:n])
+        return t.cat(cls), t.cat(prob)
+
     def save(self, path):
         with open(path, "wb") as f:
             f.write(_HDR.pack(_MAGIC, 1, self.K, self.hidden))

@@ -626,8 +626,7 @@ def predict(model_dir, test_dir, predict_dir, args, engine=None, chunk_bytes=Non
                 if batch.n and head is None:
                     cls, _ = eng.predict(batch, reverse)          # asynchronous: the kernel runs while ...
                 elif batch.n:
-                    parts = [head.predict(scores) for _, scores in batch_scores(eng, batch, reverse)]
-                    cls, prob = (eng.torch.cat(v) for v in zip(*parts))
+                    cls, prob = head.answers(batch, reverse)
             if pending is not None:
                 out.append(pending)                               # ... the previous round's lines are written
                 pending = None

@@ -176,7 +176,12 @@ def test_cli_train_and_predict_with_a_head(tmp_path, capsys):
         e.set_patterns(opal_amd.parse_patterns(f.readlines(), 64), 64)
     model_io.load_model(str(tmp_path / "headed" / "vw-model_final.model"), e)
     batch = e.ingest_fasta(np.fromfile(tmp_path / "test" / "A1.fasta", dtype=np.uint8))
-    cls, p = ScoreHead.load(e, str(tmp_path / "headed" / HEAD_FILE)).predict(e.predict(batch, True, want_scores=True)[1])
+    head = ScoreHead.load(e, str(tmp_path / "headed" / HEAD_FILE))
+    cls, p = head.answers(batch, True)
+    scores = torch.zeros(16384, K, device="cuda")
+    scores[:batch.n] = e.predict(batch, True, want_scores=True)[1]
+    direct, q = head.predict(scores)
+    assert torch.equal(cls, direct[:batch.n]) and torch.equal(p, q[:batch.n])
     assert [int(float(x.split()[0])) for x in read("p_head", "test.fragments-db.preds.vw").decode().splitlines()] == cls.tolist()
     assert ["%.6f" % x for x in p.tolist()] == read("p_head", "test.fragments-db.preds.prob").decode().split()
     e.close()
@@ -192,3 +197,59 @@ def test_cli_train_and_predict_with_a_head(tmp_path, capsys):
     assert not (tmp_path / "again" / HEAD_FILE).exists()
     with pytest.raises(ValueError, match="--head-rows"):
         train("again", "--head", "8", "--head-rows", "0")
+
+
+def _predict_rank(rank, world, port, model_dir, test_dir, out_dir):
+    import argparse
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world), LOCAL_RANK=str(rank))
+    opal.predict(model_dir, test_dir, out_dir, argparse.Namespace(kmer=64, reverse_complement=True, probabilities=True), chunk_bytes=10_000)
+
+
+@pytest.mark.gpu
+def test_answers_do_not_depend_on_pieces_or_ranks(tmp_path):
+    """A file at once, in pieces, and dealt to two ranks (both on this GPU): the same classes and probabilities, byte for byte."""
+    import argparse
+    import socket
+    import torch.multiprocessing as mp
+    import opal_amd
+    from opal_amd import model as model_io
+    rng = np.random.default_rng(29)
+    K, bits, H = 70, 18, 40
+    for d in ("model", "test"):
+        os.makedirs(tmp_path / d)
+    with open(os.path.join(os.path.dirname(os.path.abspath(__file__)), "golden", "patterns_k64_t16_m1_s7.txt")) as f:
+        (tmp_path / "model" / "patterns.txt").write_text(f.read())
+    (tmp_path / "model" / "vw-dico.txt").write_text("".join("tax%d\t%d\n" % (i, i) for i in range(1, K + 1)))
+    model_io.save_model(str(tmp_path / "model" / "vw-model_final.model"), (rng.standard_normal(1 << bits) * 0.05).astype(np.float32), K, bits)
+    params = dict(gamma=1 + 0.1 * rng.standard_normal(K), beta=0.1 * rng.standard_normal(K), w1=rng.standard_normal((H, K)) / 8, b1=rng.standard_normal(H) * 0.1,
+                  w2=rng.standard_normal((K, H)) / 6, b2=rng.standard_normal(K) * 0.1)
+    ScoreHead(HostEngine, K, H, params=params).save(str(tmp_path / "model" / HEAD_FILE))
+    with open(tmp_path / "test" / "reads.fasta", "w") as f:
+        for i in range(701):
+            f.write(">r%d\n%s\n" % (i, "".join(rng.choice(list("ACGT"), size=int(rng.integers(40, 300))))))
+    args = argparse.Namespace(kmer=64, reverse_complement=True, probabilities=True)
+    opal.predict(str(tmp_path / "model"), str(tmp_path / "test"), str(tmp_path / "one"), args)
+    opal.predict(str(tmp_path / "model"), str(tmp_path / "test"), str(tmp_path / "pieces"), args, chunk_bytes=10_000)
+    s = socket.socket()
+    s.bind(("127.0.0.1", 0))
+    port = s.getsockname()[1]
+    s.close()
+    mp.spawn(_predict_rank, args=(2, port, str(tmp_path / "model"), str(tmp_path / "test"), str(tmp_path / "two")), nprocs=2, join=True)
+    for name in ("test.fragments-db.preds.vw", "test.fragments-db.preds.taxid", "test.fragments-db.preds.prob"):
+        a = (tmp_path / "one" / name).read_bytes()
+        assert a.count(b"\n") == 701 and (tmp_path / "pieces" / name).read_bytes() == a and (tmp_path / "two" / name).read_bytes() == a
+    e = opal_amd.Engine(0)
+    with open(tmp_path / "model" / "patterns.txt") as f:
+        e.set_patterns(opal_amd.parse_patterns(f.readlines(), 64), 64)
+    model_io.load_model(str(tmp_path / "model" / "vw-model_final.model"), e)
+    head = ScoreHead.load(e, str(tmp_path / "model" / HEAD_FILE))
+    batch = e.ingest_fasta(np.fromfile(tmp_path / "test" / "reads.fasta", dtype=np.uint8))
+    cls, prob = head.answers(batch, True)
+    assert len(set(cls.tolist())) > 5
+    few = head.answers(batch, True, rows=100)                      # parts that do not divide the batch: the first is these rows alone
+    scores = e.predict(batch, True, want_scores=True)[1]
+    for lo in (0, 100):
+        part = head.predict(scores[lo:lo + 100].contiguous())
+        assert torch.equal(few[0][lo:lo + 100], part[0]) and torch.equal(few[1][lo:lo + 100], part[1])
+    assert few[0].shape == cls.shape and few[1].shape == prob.shape
+    e.close()
