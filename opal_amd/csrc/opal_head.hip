@@ -788,7 +788,7 @@ static int run_rows(opal_ctx *ctx, const Linear &product_of, int type, int produ
         return launch(q, type, product, t, dma, ctx->stream);
     };
     // 256 x 256 tiles come in rounds of one a CU.  A last round of up to a quarter of the CUs goes to smaller tiles instead, in a
-    // launch of its own: 100 000 x 1564 x 512 (3.05 rounds) 239 -> 220 us; with two fifths, 60 001 x 512 x 1563 (6.43), 312 -> 328.
+    // launch of its own: 100 000 x 512 x 1564 (3.05 rounds) 239 -> 220 us; with two fifths, 60 001 x 1563 x 512 (6.43), 245 -> 256.
     const uint64_t tn = (g.N + TILE_M[2] - 1) / TILE_M[2], tiles = tiles_of(g.M, g.N, 2), rounds = tiles / cus;
     const uint64_t rows = rounds * cus / tn * TILE_M[2];
     if (tile == 2 && rounds && rows < g.M && (tiles - rows / TILE_M[2] * tn) * 4 <= (uint64_t)cus) {
