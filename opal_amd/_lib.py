@@ -94,6 +94,18 @@ def lib():
     return _lib
 
 
+def bind():
+    """The extension module behind Engine's score head calls (csrc/opal_bind.cpp, built by __graft_entry__.build()); raises if it
+    is not there."""
+    lib()                                      # first, and with torch, which the extension is linked to
+    try:
+        from . import _bind
+    except ImportError as e:
+        raise ImportError("opal_amd/_bind.so (%s): build it with `python -c 'import __graft_entry__ as g; g.build()'`" % e) from e
+    _bind.on_error(check)
+    return _bind
+
+
 def check(rc, ctx=None):
     if rc != OPAL_OK:
         msg = lib().opal_last_error(ctx)

@@ -8,7 +8,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import check, lib
+from ._lib import bind, check, lib
 
 __all__ = ["PackedReads", "Rng", "Engine", "GenomeSet", "parse_patterns", "check_geometry"]
 
@@ -211,21 +211,20 @@ class Engine:
         torch.cuda.set_device(self.device)
         stream = torch.cuda.current_stream(self.device).cuda_stream if use_torch_stream else None
         self._stream = stream or 0
-        self._lib = lib()
+        self._lib, self._bind = lib(), bind()
         # the handle of a device's current stream: the short way where torch has it (0.1 us against 1.9)
         self._current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-        self._index, self._f32 = self.device.index, torch.float32
-        self._types = {torch.float32: _lib.OPAL_F32, torch.float16: _lib.OPAL_F16, torch.bfloat16: _lib.OPAL_BF16}
+        self._index = self.device.index
         h = C.c_void_p()
         check(lib().opal_ctx_create(device, stream, C.byref(h)))
-        self._h = h
+        self._h, self._ctx = h, h.value
         self.k = self.P = self.t = 0
         self.K = self.bits = 0
 
     def close(self):
         if getattr(self, "_h", None):
             lib().opal_ctx_destroy(self._h)
-            self._h = None
+            self._h, self._ctx = None, 0
 
     def __del__(self):
         try:
@@ -376,62 +375,14 @@ class Engine:
 
     # ------------------------------------------------------------------ score head (operators behind the per-class scores)
     # Matrices are torch tensors [n, cols] on the engine's GPU, float32 / float16 / bfloat16, whose last stride is 1 and whose row
-    # stride is at least cols (a view into wider rows is fine); new ones get rows of a multiple of 16 or 128 bytes.  The work runs on the
-    # engine's stream; when torch's current stream is another one, the two are ordered before and after the call.
-    # (What every call does is kept short: a call for one read is as long as its host side.)
-    def _matrix(self, x, name, rows=None, cols=None, dtype=None):
-        """(address, element type, row stride, rows, columns) of a matrix argument, checked."""
-        try:
-            n, c = x.shape
-            ld, one = x.stride()
-            kind = self._types[x.dtype]
-            here = x.get_device() == self._index
-        except (AttributeError, KeyError, ValueError, TypeError):
-            raise ValueError("%s must be a matrix (2-d tensor) of float32, float16 or bfloat16 on %s" % (name, self.device)) from None
-        if not here:
-            raise ValueError("%s must be on %s" % (name, self.device))
-        if dtype is not None and x.dtype != dtype:
-            raise ValueError("%s is %s: must be %s" % (name, x.dtype, dtype))
-        if (rows is not None and n != rows) or (cols is not None and c != cols):
-            raise ValueError("%s is %s: must be (%s, %s)" % (name, (n, c), "any" if rows is None else rows, "any" if cols is None else cols))
-        if n <= 1:
-            ld = c
-        if c < 1 or (one != 1 and c > 1) or ld < c:
-            raise ValueError("%s needs at least one column, columns of stride 1 and rows that do not overlap" % name)
-        return x.data_ptr(), kind, ld, n, c
-
-    def _vector(self, x, name, n, dtype=None):
-        """Address of a vector argument, checked; None for None."""
-        if x is None:
-            return None
-        try:
-            (m,) = x.shape
-            good = m == n and x.dtype is (dtype or self._f32) and x.is_contiguous() and x.get_device() == self._index
-        except (AttributeError, TypeError, ValueError):
-            good = False
-        if not good:
-            raise ValueError("%s must be a contiguous %s vector of %d on %s" % (name, dtype or self._f32, n, self.device))
-        return x.data_ptr()
-
-    def _new(self, n, cols, dtype):
-        """An uninitialised matrix: (tensor, address, element type, row stride).  Rows begin on 16 bytes, which the kernels' wide reads need;
-        rows of 1 KB or more on 128, so that a tile's part of a row is whole cache lines (60 001 x 1563 float32 logits: 273 -> 252 us)."""
-        kind = self._types.get(dtype)
-        if kind is None:
-            raise ValueError("%s: must be float32, float16 or bfloat16" % dtype)
-        each = 4 if kind == _lib.OPAL_F32 else 2
-        step = (128 if cols * each >= 1024 else 16) // each
-        ld = (cols + step - 1) & -step
-        y = self.torch.empty_strided((n, cols), (ld, 1), dtype=dtype, device=self.device)
-        return y, y.data_ptr(), kind, ld
-
-    def _run(self, call, tensors, *args):
-        """One C call on the engine's stream, ordered with torch's current stream when that is another one."""
+    # stride is at least cols (a view into wider rows is fine); new ones get rows of a multiple of 16 or 128 bytes.  Results carry no
+    # autograd history.  The work runs on the engine's stream; when torch's current stream is another one, the two are ordered
+    # before and after the call.  (A call for one read is as long as its host side: the checks of arguments, the results and
+    # workspaces are made in C++, csrc/opal_bind.cpp.)
+    def _run(self, call, tensors, *rest):
+        """One call on the engine's stream, ordered with torch's current stream when that is another one."""
         if self._current(self._index) == self._stream:
-            rc = call(self._h, *args)
-            if rc:
-                check(rc, self._h)
-            return
+            return call(self._ctx, self._index, *tensors, *rest)
         t = self.torch
         cur = t.cuda.current_stream(self.device)
         if t.cuda.is_current_stream_capturing():
@@ -439,109 +390,49 @@ class Engine:
         # (an ExternalStream of handle 0 would be a new stream, not the default one)
         own = t.cuda.ExternalStream(self._stream, device=self.device) if self._stream else t.cuda.default_stream(self.device)
         own.wait_stream(cur)
-        check(call(self._h, *args), self._h)
+        # what the call allocates comes from the current stream's memory and goes back to it: later work there waits for the engine's
+        out = call(self._ctx, self._index, *tensors, *rest)
         cur.wait_stream(own)
-        for x in tensors:                      # their memory may be handed out again once the engine's stream is done with it
+        for x in (*tensors, *out):             # their memory may be handed out again once the engine's stream is done with it
             if x is not None:
                 x.record_stream(own)
+        return out
 
     def layer_norm(self, x, gamma=None, beta=None, eps=1e-5, out_dtype=None, want_stats=False):
         """y = (x - mean) rstd gamma + beta per row (opal_layer_norm).  Returns (y, mean, rstd); mean and rstd are None unless
         want_stats (layer_norm_backward needs them).  out_dtype: of y, default that of x."""
-        px, tx, ldx, n, cols = self._matrix(x, "x")
-        pg, pb = self._vector(gamma, "gamma", cols), self._vector(beta, "beta", cols)
-        y, py, ty, ldy = self._new(n, cols, out_dtype or x.dtype)
-        mean = rstd = pm = pr = None
-        if want_stats:
-            t = self.torch
-            mean, rstd = t.empty(n, dtype=t.float32, device=self.device), t.empty(n, dtype=t.float32, device=self.device)
-            pm, pr = mean.data_ptr(), rstd.data_ptr()
-        self._run(self._lib.opal_layer_norm, (x, gamma, beta, y, mean, rstd), px, tx, ldx, pg, pb, n, cols, eps, py, ty, ldy, pm, pr)
-        return y, mean, rstd
+        return self._run(self._bind.layer_norm, (x, gamma, beta), eps, out_dtype, want_stats)
 
     def layer_norm_backward(self, dy, x, gamma, mean, rstd, out_dtype=None, want_dx=True, want_params=True):
         """The gradients of layer_norm: (dx, dgamma, dbeta) (opal_layer_norm_backward); those not wanted are None.  gamma may be
         None (= 1).  out_dtype: of dx, default that of x."""
-        t = self.torch
-        px, tx, ldx, n, cols = self._matrix(x, "x")
-        pd, td, ldd, _, _ = self._matrix(dy, "dy", n, cols)
-        pg, pm, pr = self._vector(gamma, "gamma", cols), self._vector(mean, "mean", n), self._vector(rstd, "rstd", n)
-        if pm is None or pr is None:
-            raise ValueError("mean and rstd of the forward pass are needed (layer_norm(..., want_stats=True))")
-        dx, px_out, tx_out, lddx = self._new(n, cols, out_dtype or x.dtype) if want_dx else (None, None, 0, 0)
-        dg = db = work = None
-        size = 0
-        if want_params:
-            dg, db = t.empty(cols, dtype=t.float32, device=self.device), t.empty(cols, dtype=t.float32, device=self.device)
-            size = self._lib.opal_layer_norm_backward_workspace(n, cols)
-            work = t.empty(size, dtype=t.uint8, device=self.device) if size else None
-        self._run(self._lib.opal_layer_norm_backward, (dy, x, gamma, mean, rstd, dx, dg, db, work), pd, td, ldd, px, tx, ldx, pg, pm, pr, n, cols, px_out, tx_out,
-                  lddx, dg.data_ptr() if want_params else None, db.data_ptr() if want_params else None, work.data_ptr() if size else None, size)
-        return dx, dg, db
+        return self._run(self._bind.layer_norm_backward, (dy, x, gamma, mean, rstd), out_dtype, want_dx, want_params)
 
     def linear(self, x, w, bias=None, activation="none", residual=None, out_dtype=None, want_pre=False):
         """y = act(x w^T + bias) + residual (opal_linear): x [n, in] and w [out, in] of one type, bias float32 [out], activation
         none / relu / silu / gelu (tanh form), residual [n, out] of any type.  Returns (y, pre); pre, the value before the
         activation in the type of x (linear_grad_input takes it), is None unless want_pre.  out_dtype: of y, default that of x."""
-        px, tx, ldx, n, k = self._matrix(x, "x")
-        pw, _, ldw, m, _ = self._matrix(w, "w", None, k, x.dtype)
-        act = self._activation(activation)
-        pb = self._vector(bias, "bias", m)
-        pr, tr, ldr, _, _ = self._matrix(residual, "residual", n, m) if residual is not None else (None, 0, 0, 0, 0)
-        y, py, ty, ldy = self._new(n, m, out_dtype or x.dtype)
-        pre, pp, _, ldp = self._new(n, m, x.dtype) if want_pre else (None, None, 0, 0)
-        self._run(self._lib.opal_linear, (x, w, bias, residual, y, pre), px, ldx, pw, ldw, tx, pb, act, pr, tr, ldr, n, k, m, py, ty, ldy, pp, ldp)
-        return y, pre
+        return self._run(self._bind.linear, (x, w, bias, residual), self._activation(activation), out_dtype, want_pre)
 
     def linear_grad_input(self, dy, w, pre=None, activation="none", residual=None, out_dtype=None):
         """dx = (dy w) act'(pre) + residual (opal_linear_grad_input): dy [n, out] and w [out, in] of one type, pre [n, in] the value
         before the activation that made the product's input (needed unless activation is none), residual [n, in] the gradient
         that reaches the input past the product.  out_dtype: of dx, default that of dy."""
-        pd, td, ldd, n, m = self._matrix(dy, "dy")
-        pw, _, ldw, _, k = self._matrix(w, "w", m, None, dy.dtype)
-        act = self._activation(activation)
-        if act and pre is None:
-            raise ValueError("an activation's gradient needs pre (linear(..., want_pre=True))")
-        pp, _, ldp, _, _ = self._matrix(pre, "pre", n, k, dy.dtype) if act else (None, 0, 0, 0, 0)
-        pr, tr, ldr, _, _ = self._matrix(residual, "residual", n, k) if residual is not None else (None, 0, 0, 0, 0)
-        dx, px, tx, ldx = self._new(n, k, out_dtype or dy.dtype)
-        self._run(self._lib.opal_linear_grad_input, (dy, w, pre, residual, dx), pd, ldd, pw, ldw, td, pp, ldp, act, pr, tr, ldr, n, k, m, px, tx, ldx)
-        return dx
+        return self._run(self._bind.linear_grad_input, (dy, w, pre, residual), self._activation(activation), out_dtype)[0]
 
     def linear_grad_weight(self, dy, x, want_bias=True):
         """(dw, dbias) = (dy^T x, sum of dy's rows), float32 (opal_linear_grad_weight): dy [n, out] and x [n, in] of one type."""
-        t = self.torch
-        px, tx, ldx, n, k = self._matrix(x, "x")
-        pd, _, ldd, _, m = self._matrix(dy, "dy", n, None, x.dtype)
-        dw = t.empty((m, k), dtype=t.float32, device=self.device)
-        db = t.empty(m, dtype=t.float32, device=self.device) if want_bias else None
-        size = self._lib.opal_linear_grad_weight_workspace(n, k, m, tx)
-        work = t.empty(size, dtype=t.uint8, device=self.device) if size else None
-        self._run(self._lib.opal_linear_grad_weight, (dy, x, dw, db, work), pd, ldd, px, ldx, tx, n, k, m, dw.data_ptr(), k,
-                  db.data_ptr() if want_bias else None, work.data_ptr() if size else None, size)
-        return dw, db
+        return self._run(self._bind.linear_grad_weight, (dy, x), want_bias)
 
     def softmax_loss(self, scores, labels, scale=1.0, out_dtype=None, want_grad=True):
         """Cross entropy of each row's softmax against its class id (opal_softmax_loss): labels int32 [n], 1..K, 0 = no known class
         (loss and gradient 0).  Returns (loss float32 [n], scale times the gradient [n, K] or None).  out_dtype: of the gradient,
         default that of scores."""
-        t = self.torch
-        ps, ts, lds, n, K = self._matrix(scores, "scores")
-        pl = self._vector(labels, "labels", n, t.int32)
-        if pl is None:
-            raise ValueError("labels are needed")
-        loss = t.empty(n, dtype=t.float32, device=self.device)
-        grad, pg, tg, ldg = self._new(n, K, out_dtype or scores.dtype) if want_grad else (None, None, 0, 0)
-        self._run(self._lib.opal_softmax_loss, (scores, labels, loss, grad), ps, ts, lds, n, K, pl, scale, loss.data_ptr(), pg, tg, ldg)
-        return loss, grad
+        return self._run(self._bind.softmax_loss, (scores, labels), scale, out_dtype, want_grad)
 
     def softmax_class(self, scores):
         """(class int32 [n], 1-based as from predict, its softmax probability float32 [n]) of the highest score of each row."""
-        t = self.torch
-        ps, ts, lds, n, K = self._matrix(scores, "scores")
-        cls, prob = t.empty(n, dtype=t.int32, device=self.device), t.empty(n, dtype=t.float32, device=self.device)
-        self._run(self._lib.opal_softmax_class, (scores, cls, prob), ps, ts, lds, n, K, cls.data_ptr(), prob.data_ptr())
-        return cls, prob
+        return self._run(self._bind.softmax_class, (scores,))
 
     def _activation(self, name):
         if name not in ACTIVATIONS:
