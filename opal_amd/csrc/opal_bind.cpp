@@ -32,8 +32,12 @@ struct Env {
     opal_ctx *ctx;
     int index;                                 // of the GPU
     at::TensorOptions on(at::ScalarType s) const { return at::TensorOptions().dtype(s).device(at::Device(at::kCUDA, (c10::DeviceIndex)index)); }
-    void done(int rc) const
+    // A C entry, without the interpreter's lock (a launch waits when the queue is full); its status raises.
+    template <class F> void run(F &&entry) const
     {
+        PyThreadState *state = PyEval_SaveThread();
+        const int rc = entry();
+        PyEval_RestoreThread(state);
         if (rc == OPAL_OK) return;
         PyObject *r = PyObject_CallFunction(check, "iK", rc, (unsigned long long)(uintptr_t)ctx);
         Py_XDECREF(r);
@@ -41,6 +45,9 @@ struct Env {
         throw Failed();
     }
 };
+
+// sizes as the C entries take them: what does not fit is larger than they allow, and stays so
+uint32_t u32(int64_t v) { return v > 0xffffffffll ? 0xffffffffu : (uint32_t)v; }
 
 struct Matrix {
     void *p = nullptr;
@@ -164,8 +171,8 @@ PyObject *layer_norm(const Env &e, PyObject *const *a)
         mean = new_vector(e, x.rows);
         rstd = new_vector(e, x.rows);
     }
-    e.done(opal_layer_norm(e.ctx, x.p, x.type, x.ld, (const float *)gamma, (const float *)beta, x.rows, (uint32_t)x.cols, eps, at_of(y), type, ld_of(y),
-                           (float *)at_of(mean), (float *)at_of(rstd)));
+    e.run([&] { return opal_layer_norm(e.ctx, x.p, x.type, x.ld, (const float *)gamma, (const float *)beta, x.rows, u32(x.cols), eps, at_of(y), type, ld_of(y),
+                           (float *)at_of(mean), (float *)at_of(rstd)); });
     return results(y, mean, rstd);
 }
 
@@ -182,11 +189,11 @@ PyObject *layer_norm_backward(const Env &e, PyObject *const *a)
     if (is_true(a[7])) {
         dgamma = new_vector(e, x.cols);
         dbeta = new_vector(e, x.cols);
-        bytes = opal_layer_norm_backward_workspace(x.rows, (uint32_t)x.cols);
+        bytes = opal_layer_norm_backward_workspace(x.rows, u32(x.cols));
         if (bytes) work = new_vector(e, (int64_t)bytes, at::kByte);
     }
-    e.done(opal_layer_norm_backward(e.ctx, dy.p, dy.type, dy.ld, x.p, x.type, x.ld, (const float *)gamma, (const float *)mean, (const float *)rstd, x.rows,
-                                    (uint32_t)x.cols, at_of(dx), type, ld_of(dx), (float *)at_of(dgamma), (float *)at_of(dbeta), at_of(work), bytes));
+    e.run([&] { return opal_layer_norm_backward(e.ctx, dy.p, dy.type, dy.ld, x.p, x.type, x.ld, (const float *)gamma, (const float *)mean, (const float *)rstd, x.rows,
+                                    u32(x.cols), at_of(dx), type, ld_of(dx), (float *)at_of(dgamma), (float *)at_of(dbeta), at_of(work), bytes); });
     return results(dx, dgamma, dbeta);
 }
 
@@ -200,8 +207,8 @@ PyObject *linear(const Env &e, PyObject *const *a)
     const at::Tensor y = new_matrix(e, x.rows, w.rows, type);
     at::Tensor pre;
     if (is_true(a[6])) pre = new_matrix(e, x.rows, w.rows, x.type);
-    e.done(opal_linear(e.ctx, x.p, x.ld, w.p, w.ld, x.type, (const float *)bias, act, res.p, res.type, res.ld, x.rows, (uint32_t)x.cols, (uint32_t)w.rows,
-                       at_of(y), type, ld_of(y), at_of(pre), ld_of(pre)));
+    e.run([&] { return opal_linear(e.ctx, x.p, x.ld, w.p, w.ld, x.type, (const float *)bias, act, res.p, res.type, res.ld, x.rows, u32(x.cols), u32(w.rows),
+                       at_of(y), type, ld_of(y), at_of(pre), ld_of(pre)); });
     return results(y, pre);
 }
 
@@ -214,8 +221,8 @@ PyObject *linear_grad_input(const Env &e, PyObject *const *a)
     const Matrix pre = act ? matrix(e, a[2], "pre", dy.rows, w.cols, dy.type) : Matrix();
     const Matrix res = optional_matrix(e, a[3], "residual", dy.rows, w.cols);
     const at::Tensor dx = new_matrix(e, dy.rows, w.cols, type);
-    e.done(opal_linear_grad_input(e.ctx, dy.p, dy.ld, w.p, w.ld, dy.type, pre.p, pre.ld, act, res.p, res.type, res.ld, dy.rows, (uint32_t)w.cols,
-                                  (uint32_t)dy.cols, at_of(dx), type, ld_of(dx)));
+    e.run([&] { return opal_linear_grad_input(e.ctx, dy.p, dy.ld, w.p, w.ld, dy.type, pre.p, pre.ld, act, res.p, res.type, res.ld, dy.rows, u32(w.cols),
+                                  u32(dy.cols), at_of(dx), type, ld_of(dx)); });
     return results(dx);
 }
 
@@ -226,10 +233,10 @@ PyObject *linear_grad_weight(const Env &e, PyObject *const *a)
     const at::Tensor dw = at::empty({dy.cols, x.cols}, e.on(at::kFloat));
     at::Tensor db, work;
     if (is_true(a[2])) db = new_vector(e, dy.cols);
-    const uint64_t bytes = opal_linear_grad_weight_workspace(x.rows, (uint32_t)x.cols, (uint32_t)dy.cols, x.type);
+    const uint64_t bytes = opal_linear_grad_weight_workspace(x.rows, u32(x.cols), u32(dy.cols), x.type);
     if (bytes) work = new_vector(e, (int64_t)bytes, at::kByte);
-    e.done(opal_linear_grad_weight(e.ctx, dy.p, dy.ld, x.p, x.ld, x.type, x.rows, (uint32_t)x.cols, (uint32_t)dy.cols, (float *)at_of(dw), (uint64_t)x.cols,
-                                   (float *)at_of(db), at_of(work), bytes));
+    e.run([&] { return opal_linear_grad_weight(e.ctx, dy.p, dy.ld, x.p, x.ld, x.type, x.rows, u32(x.cols), u32(dy.cols), (float *)at_of(dw), (uint64_t)x.cols,
+                                   (float *)at_of(db), at_of(work), bytes); });
     return results(dw, db);
 }
 
@@ -244,7 +251,7 @@ PyObject *softmax_loss(const Env &e, PyObject *const *a)
     const at::Tensor loss = new_vector(e, s.rows);
     at::Tensor grad;
     if (is_true(a[4])) grad = new_matrix(e, s.rows, s.cols, type);
-    e.done(opal_softmax_loss(e.ctx, s.p, s.type, s.ld, s.rows, (uint32_t)s.cols, (const int32_t *)labels, scale, (float *)at_of(loss), at_of(grad), type, ld_of(grad)));
+    e.run([&] { return opal_softmax_loss(e.ctx, s.p, s.type, s.ld, s.rows, u32(s.cols), (const int32_t *)labels, scale, (float *)at_of(loss), at_of(grad), type, ld_of(grad)); });
     return results(loss, grad);
 }
 
@@ -253,7 +260,7 @@ PyObject *softmax_class(const Env &e, PyObject *const *a)
 {
     const Matrix s = matrix(e, a[0], "scores");
     const at::Tensor cls = new_vector(e, s.rows, at::kInt), prob = new_vector(e, s.rows);
-    e.done(opal_softmax_class(e.ctx, s.p, s.type, s.ld, s.rows, (uint32_t)s.cols, (int32_t *)at_of(cls), (float *)at_of(prob)));
+    e.run([&] { return opal_softmax_class(e.ctx, s.p, s.type, s.ld, s.rows, u32(s.cols), (int32_t *)at_of(cls), (float *)at_of(prob)); });
     return results(cls, prob);
 }
 

@@ -679,7 +679,8 @@ def test_engine_refuses(eng):
         with pytest.raises(ValueError):
             call()
     import opal_amd
-    for call in (lambda: eng.layer_norm(x, eps=0.0), lambda: eng.layer_norm(x, eps=float("nan"))):
+    long = torch.zeros((1 << 20) + 1, 8, device="cuda")           # more outputs than a product has
+    for call in (lambda: eng.layer_norm(x, eps=0.0), lambda: eng.layer_norm(x, eps=float("nan")), lambda: eng.linear(x[:1], long), lambda: eng.softmax_class(long.view(1, -1)[:, :(1 << 20) + 1])):
         with pytest.raises(opal_amd.OpalError):
             call()
 
