@@ -515,8 +515,9 @@ template <class T> static void run_softmax(const Softmax &g, int cus, hipStream_
 #undef L
 }
 
-// Blocks of the backward pass, which is the number of partial sums: enough waves to fill the card (two blocks a CU), and none with
-// less than four rows a team, below which the partial sums would be as much to read as the rows.
+// Blocks of the backward pass, which is the number of partial sums.  Many rows: enough waves to fill the card (two blocks a CU), four rows a
+// team at least, below which the partial sums would be as much to read as the rows.  Few: a row a team, since rows in turn are 2 us each: 500 x 356
+// 10.4 us a call against 15.8 with four, 5000 x 356 12.0 against 17.5.  Up to two rows a team: one block (64 x 356 9.6 against 10.2).
 constexpr uint64_t NORM_BACK_BLOCKS = 512;
 static uint64_t norm_back_blocks(uint64_t n, uint32_t cols)
 {
@@ -525,9 +526,10 @@ static uint64_t norm_back_blocks(uint64_t n, uint32_t cols)
     uint64_t rows;
     OPAL_TEAMS(ROWS, cols)
 #undef ROWS
-    return std::min<uint64_t>((n + 4 * rows - 1) / (4 * rows), cols <= 2048 ? NORM_BACK_BLOCKS : 2 * NORM_BACK_BLOCKS);
+    if (n <= 2 * rows) return n > 0;
+    return std::max(std::min<uint64_t>((n + rows - 1) / rows, 256), std::min<uint64_t>((n + 4 * rows - 1) / (4 * rows), cols <= 2048 ? NORM_BACK_BLOCKS : 2 * NORM_BACK_BLOCKS));
 }
-// One block needs no sum behind it, and no workspace: 100 x 356 11.6 us a call against 15.3.
+// One block needs no sum behind it, and no workspace.
 static bool norm_back_alone(uint64_t n, uint32_t cols) { return cols <= BLOCK_COLS && norm_back_blocks(n, cols) == 1; }
 
 template <class TX, class TY> static void run_norm_back(const NormBack &g, unsigned blocks, int cus, hipStream_t st)
