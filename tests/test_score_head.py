@@ -709,3 +709,17 @@ def test_workspace_sizes():
     for n in (1, 100, 10 ** 6):
         for k, m in ((1, 1), (355, 63), (1564, 512)):
             assert L.opal_linear_grad_weight_workspace(n, k, m, 2) < 1 << 30
+
+
+def test_binding_refuses_without_a_gpu():
+    """The extension module loads where there is no GPU, and refuses what is no matrix on one."""
+    from opal_amd._lib import bind
+    b = bind()
+    x = torch.zeros(2, 8)
+    for call in (lambda: b.softmax_class(0, 0, x), lambda: b.softmax_class(0, 0, None), lambda: b.softmax_class(0, 0, [1.0]), lambda: b.linear(0, 0, x, x, None, None, 0, None, False),
+                 lambda: b.layer_norm(0, 0, x.double(), None, None, 1e-5, None, False), lambda: b.linear_grad_weight(0, 0, x[0], x, True)):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: b.softmax_class(0, 0), lambda: b.linear(0, 0, x, x), lambda: b.softmax_class("ctx", 0, x)):
+        with pytest.raises(TypeError):
+            call()
