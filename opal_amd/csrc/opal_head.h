@@ -170,7 +170,6 @@ __device__ __forceinline__ void wave_order()
     __builtin_amdgcn_wave_barrier();
 }
 
-inline int type_bytes(int type) { return type == OPAL_F32 ? 4 : 2; }
 inline bool type_ok(int type) { return type == OPAL_F32 || type == OPAL_F16 || type == OPAL_BF16; }
 
 // makes the ctx's device current for a call and puts the caller's back

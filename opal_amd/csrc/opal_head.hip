@@ -695,44 +695,6 @@ static hipError_t launch(const Linear &g, int type, int product, int tile, bool 
     return launch_linear<bf16_t>(g, product, tile, dma, st);
 }
 
-constexpr int TILE_M[] = {64, 128, 256, 0, 128, 32}, TILE_N[] = {64, 128, 256, 0, 256, 32};
-
-static uint64_t tiles_of(uint64_t M, uint64_t N, int tile) { return ((M + TILE_M[tile] - 1) / TILE_M[tile]) * ((N + TILE_N[tile] - 1) / TILE_N[tile]); }
-
-// Larger tiles read fewer bytes for the same sums, smaller ones leave fewer CUs idle and less of a tile outside the matrix (us; rows x N x K):
-//   128 x 128 instead of 64 x 64, 16-bit types, sums of 512 on, from 1.5 tiles a CU on: 16384 x 1564 x 512 34.5 against 49.3, 100 000 x 128 x 1000 49
-//   against 56; below it 4096 x 1564 x 512 (416) 14.4 against 15.1; shorter sums 100 000 x 200 x 200 24.4 against 21.8.  Not where it reaches a
-//   quarter further: 100 000 x 150 x 1000 90 against 83, 100 000 x 64 x 512 26 against 20.  32-bit types, bound by the matrix pipe, never: 50 000 x
-//   512 x 1564 694 against 674, 100 000 x 200 x 150 126 against 82.
-// 16-bit types, aligned:
-//   256 x 256 from one tile a CU on.  Input gradients where it does not reach a quarter further than 128 x 128: 32768 x 512 x 256 17.5 against 22.3, 100 000 x
-//   600 x 64 35 against 44; but 100 000 x 356 x 1000 125 against 113.  Forward products, which have 128 x 256 tiles too, with more than
-//   128 columns and sums of 1024 on (32768 x 512 x 1564 (256) 51 against 59; below it 16384 x 512 x 1564 (128) 38 against 32), or of 256 on from
-//   four tiles a CU on: 250 000 x 355 x 256 (1954) 106 against 110, 100 000 x 1563 x 256 140 against 169; below it 100 000 x 512 x 512 (782) 76
-//   against 70, 32768 x 1564 x 512 (896) 72 against 68.
-//   128 x 256 (forward, more than 128 columns) from 3/4 of a tile a CU on: 250 000 x 355 x 128 66 against 82 with 256 x 256 and 104 with 128 x 128, 4096 x
-//   1564 x 512 (224) 14.1 against 15.5; below it 4099 x 512 x 355 (66) 12.2 against 10.9, 16384 x 200 x 200 (128) 10.9 against 7.7.
-// large: the last two may take it; whole: the first of them too.
-static uint64_t reach(uint64_t N, uint64_t tile) { return (N + tile - 1) / tile * tile; }
-static int pick_tile(int product, int type, uint64_t M, uint64_t N, uint64_t K, int cus, bool large, bool whole)
-{
-    const uint64_t c = cus, t256 = tiles_of(M, N, 2);
-    if (large && whole && t256 >= c &&
-        (product == FWD ? N > 128 && (K >= 1024 || (K >= 256 && t256 >= 4 * c)) : reach(N, 256) * 4 <= reach(N, 128) * 5)) return 2;
-    if (large && product == FWD && N > 128 && tiles_of(M, N, 4) * 4 >= 3 * c) return 4;
-    return type != OPAL_F32 && K >= 512 && tiles_of(M, N, 1) * 2 >= 3 * c && reach(N, 128) * 4 <= reach(N, 64) * 5 ? 1 : 0;
-}
-
-// The kernel for few rows, while its blocks (64 x 16 results, all of k) find a CU each (rows x N x K): 16-bit types 64 x 512 x 1564 8.1 us against 10.3
-// with 64 x 64 tiles, 1024 rows 12.6 against 10.7; an input gradient, which gathers W's columns there one by one, up to 16 rows (9.9
-// against 10.5; 100 rows 13.5 against 10.9).  32-bit types, whose tiles are bound by a wave's chain of MFMAs, both: 512 x 512 x 1564 19
-// against 36, input gradients of 2048 x 100 x 356 6.4 against 10.5; 600 x 1000 x 4000 (630 blocks) 128 against 86.
-static bool few_rows(int product, int type, uint64_t M, uint64_t N, int cus)
-{
-    if (product == GIN && M > 16 && type != OPAL_F32) return false;
-    return ((M + 63) / 64) * ((N + 15) / 16) <= (uint64_t)cus;
-}
-
 static void set_tiles(Linear &g, int tile)
 {
     g.tm = (uint32_t)((g.M + TILE_M[tile] - 1) / TILE_M[tile]);
@@ -776,7 +738,7 @@ static int run_rows(opal_ctx *ctx, const Linear &product_of, int type, int produ
     const int cus = ctx->num_cus;
     // (the two kernels for large products write 32 bits or the operands' type, and read such a residual)
     const bool large = dma && type != OPAL_F32 && (g.y_type == OPAL_F32 || g.y_type == type) && (!g.res || g.res_type == OPAL_F32 || g.res_type == type);
-    int tile = few_rows(product, type, g.M, g.N, cus) ? 3 : pick_tile(product, type, g.M, g.N, g.K, cus, large, true);
+    int tile = product_tile(product, type, g.M, g.N, g.K, cus, large, true);
     g.splits = 1;
     g.ksplit = g.K;
     auto run = [&](Linear &q, int t) {
@@ -798,7 +760,7 @@ static int run_rows(opal_ctx *ctx, const Linear &product_of, int type, int produ
         q.M = rows;
         OPAL_HIP_CHECK(ctx, run(q, 2));
         g = behind(g, rows, type);
-        tile = few_rows(product, type, g.M, g.N, cus) ? 3 : pick_tile(product, type, g.M, g.N, g.K, cus, large, false);
+        tile = product_tile(product, type, g.M, g.N, g.K, cus, large, false);
     }
     OPAL_HIP_CHECK(ctx, run(g, tile));
     return OPAL_OK;
@@ -856,28 +818,6 @@ extern "C" int opal_linear_grad_input(opal_ctx *ctx, const void *d_dy, uint64_t 
     g.res = d_res; g.res_type = res_type; g.ldr = ldr;
     g.y = d_dx; g.y_type = dx_type; g.ldy = lddx;
     return run_rows(ctx, g, type, GIN);
-}
-
-// Splits of the sum over the rows, none empty.  256 x 256 tiles: as many as give the 256 CUs a tile each, of at least 16 steps.
-// Smaller ones: two blocks per CU, of at least four steps; 128 x 128 from twelve on: 20 000 x 512 x 512 (16 tiles) 16.3 us against 22.3 with 64 x
-// 64, 6000 x 1564 x 512 (52) 16.8 against 22.0; below it 8192 x 512 x 256 (8) 9.2 against 7.1, 20 000 x 355 x 128 (3) 12.1 against 7.5.  Few rows, while 32 x 32 tiles find a CU each, are one block's for all of the
-// sum, without splits to add up: 1999 x 355 x 63 (rows, in, out) 5.3 us against 4.8 and 4.6 for the splits' sum; 4096 x 355 x 128 8.8 against
-// 10.2 + 4.6, 8192 x 355 x 128 26 against 10.6 + 4.6; 32-bit types, whose operands are loads of one column, 1024 x 512 x 512 10.0 against 13.6 +
-// 4.6, 1024 x 384 x 64 9.8 against 5.5 + 4.6, 1999 x 355 x 63 15.7 against 5.9 + 4.6.  The choice does not look at the operands' alignment, so that the workspace
-// does not depend on it; unaligned operands take 128 x 128 tiles in the same splits.
-struct Splits { int tile; uint64_t splits, rows; };
-static Splits weight_splits(uint64_t n, uint32_t in, uint32_t out, int type)
-{
-    if (n <= (type == OPAL_F32 ? 1024 : 4096) && tiles_of(out, in, 5) <= 256) return {5, 1, n};
-    const uint64_t step = STEP_BYTES / type_bytes(type);
-    const uint64_t steps = std::max<uint64_t>((n + step - 1) / step, 1);
-    const uint64_t big = tiles_of(out, in, 2);
-    const bool large = type != OPAL_F32 && in > 128 && out > 128 && steps * big >= 16 * 128;
-    const int tile = large ? 2 : in > 64 && out > 64 && tiles_of(out, in, 1) >= 12 ? 1 : 0;
-    uint64_t s = large ? std::min<uint64_t>(256 / std::min<uint64_t>(big, 256), steps / 16) : std::min<uint64_t>(512 / std::min<uint64_t>(tiles_of(out, in, tile), 512), steps / 4);
-    s = std::max<uint64_t>(s, 1);
-    const uint64_t per = (steps + s - 1) / s;
-    return {tile, (steps + per - 1) / per, per * step};
 }
 
 extern "C" uint64_t opal_linear_grad_weight_workspace(uint64_t n, uint32_t in, uint32_t out, int type)

@@ -14,10 +14,10 @@
 // 16384 x 200 x 200 8 us; 100 000 x 128 x 1000 with 128 x 128 tiles 49 us, 525 TFLOP/s.
 #pragma once
 #include "opal_head.h"
+#include "opal_linear_rules.h"
 
 namespace opal_head {
 
-enum Product { FWD = 0, GIN = 1, GWT = 2 };
 enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
 struct Linear {
@@ -75,8 +75,6 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
-
-constexpr int STEP_BYTES = 128;          // of k per row and step
 
 // Where chunk c of row r of a KC tile lies within the row's eight: rows r and r + 1 share 256 bytes (all banks), the rotation by
 // r >> 1 then spreads the same c of 16 rows over all 16 places, which is what a fragment read asks for.
@@ -667,8 +665,7 @@ template <class T> __global__ __launch_bounds__(FEWW_WAVES * WAVE) void linear_f
     }
 }
 
-// The launch of one product in one element type (opal_linear_{f32,f16,bf16}.hip); tile: 0 = 64 x 64, 1 = 128 x 128, 2 = 256 x 256
-// (16-bit types on the aligned path only), 3 = few rows (g.few x 16), 4 = 128 x 256 (FWD, as 2), 5 = 32 x 32 over all rows (GWT).
+// The launch of one product in one element type (opal_linear_{f32,f16,bf16}.hip); tile: opal_linear_rules.h.
 template <class T> hipError_t launch_linear(const Linear &g, int product, int tile, bool dma, hipStream_t stream);
 
 #define OPAL_LINEAR_CASE(T, P, TILE, BM, BN, WM, WN, D)                                                                              \
