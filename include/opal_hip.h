@@ -301,7 +301,7 @@ int opal_softmax_loss(opal_ctx *ctx, const void *d_scores, int type, uint64_t ld
                       float scale, float *d_loss, void *d_grad, int grad_type, uint64_t ldg);
 
 /* The answer: d_out_class[i] = 1-based class of the highest score (ties: the lowest class; NaN never wins; class 1 when nothing is
- * above -inf), d_out_prob[i] (may be NULL) = its softmax probability (0 when nothing is above -inf).                   */
+ * above -inf), d_out_prob[i] (may be NULL) = its softmax probability (0 when all scores are -inf; NaN where one is NaN or +inf). */
 int opal_softmax_class(opal_ctx *ctx, const void *d_scores, int type, uint64_t ld, uint64_t n, uint32_t K, int32_t *d_out_class, float *d_out_prob);
 
 /* Name of the scoring-kernel variant opal_predict would launch for the current K (for profiles/bench).   */

@@ -391,7 +391,7 @@ template <class T, int TPR, int NQ, bool NT> __global__ __launch_bounds__(BLOCK)
             for (int e = 3; e >= 0; e--)
                 if (x[i][e] == top) first = quad_col<TPR, NQ>(i, t) + e;
         const float low = -team.max(first == 0x7fffffff ? -INFINITY : -(float)first);   // cols <= 2^20: exact in a float
-        best = low < (float)g.cols ? (int)low : 0;
+        best = top > -INFINITY && low < (float)g.cols ? (int)low : 0;      // -inf is ruled out, behind a NaN too: class 1 then
     }
     const float shift = top == -INFINITY ? 0.f : top;
     float z = 0.f;
@@ -448,7 +448,7 @@ template <class T> __global__ __launch_bounds__(LONG) void softmax_long_kernel(c
                 store4_typed(g.grad, g.grad_type, row * g.ldg + c, 1, f32x4{!none && c == label ? p - g.scale : p, 0.f, 0.f, 0.f});
             }
         }
-        if (threadIdx.x == 0) softmax_row(g, row, shift, z, low < (float)g.cols ? (int)low : 0, label, bad, at);
+        if (threadIdx.x == 0) softmax_row(g, row, shift, z, top > -INFINITY && low < (float)g.cols ? (int)low : 0, label, bad, at);
     }
 }
 

@@ -1,0 +1,39 @@
+"""Calls of the score head that its documentation allows at the edges of what it says: rows without a class, odd tensors, other streams, empty
+batches.  (test_score_head.py holds the operators against their formulas.)"""
+import os
+import sys
+
+import pytest
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+import torch  # noqa: E402
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def eng():
+    import opal_amd
+    e = opal_amd.Engine(0)
+    yield e
+    e.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [1, 2, 10, 300, 2500, 9000])
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+def test_class_one_when_nothing_is_above_minus_infinity(eng, t, K):
+    """NaN never wins, and a class at -inf is ruled out: also where a NaN stands before it the answer is class 1."""
+    inf, nan = float("inf"), float("nan")
+    s = torch.full((6, K), -inf)
+    s[1, 0] = nan
+    s[2, : K // 2 + 1] = nan
+    s[3] = nan
+    s[4, K - 1] = nan
+    s[5, 0] = nan
+    s[5, K - 1] = torch.finfo(t).min           # the lowest number is above -inf
+    cls, prob = eng.softmax_class(s.to(t).cuda())
+    assert cls.tolist() == [1, 1, 1, 1, 1, K]
+    prob = prob.cpu()
+    assert prob[0] == 0 and prob[1:5].isnan().all()
+    assert prob[5] == 1 if K == 1 else prob[5].isnan()
