@@ -124,7 +124,12 @@ template <class... T> PyObject *results(const T &...t)
     return r;
 }
 
-bool is_true(PyObject *o) { return PyObject_IsTrue(o) == 1; }
+bool is_true(PyObject *o)
+{
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw Failed();
+    return v == 1;
+}
 double number(PyObject *o)
 {
     const double v = PyFloat_AsDouble(o);

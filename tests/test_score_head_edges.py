@@ -37,3 +37,17 @@ def test_class_one_when_nothing_is_above_minus_infinity(eng, t, K):
     prob = prob.cpu()
     assert prob[0] == 0 and prob[1:5].isnan().all()
     assert prob[5] == 1 if K == 1 else prob[5].isnan()
+
+
+@pytest.mark.gpu
+def test_a_flag_without_a_truth_value_raises_its_own_error(eng):
+    class Neither:
+        def __bool__(self):
+            raise LookupError("neither")
+    x, w = torch.randn(4, 8, device="cuda"), torch.randn(6, 8, device="cuda")
+    one, labels = torch.ones(4, device="cuda"), torch.ones(4, dtype=torch.int32, device="cuda")
+    for call in (lambda f: eng.layer_norm(x, want_stats=f), lambda f: eng.layer_norm_backward(x, x, None, one, one, want_dx=f),
+                 lambda f: eng.layer_norm_backward(x, x, None, one, one, want_params=f), lambda f: eng.linear(x, w, want_pre=f),
+                 lambda f: eng.linear_grad_weight(x, x, want_bias=f), lambda f: eng.softmax_loss(x, labels, want_grad=f)):
+        with pytest.raises(LookupError, match="neither"):
+            call(Neither())
