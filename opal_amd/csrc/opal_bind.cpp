@@ -63,6 +63,7 @@ Matrix matrix(const Env &e, PyObject *o, const char *name, int64_t rows = -1, in
     const int kind = t ? type_of(t->scalar_type()) : -1;
     if (kind < 0 || t->layout() != at::kStrided || t->dim() != 2)
         refuse("%s must be a matrix (2-d tensor) of float32, float16 or bfloat16 on cuda:%d", name, e.index);
+    if (t->is_neg()) refuse("%s is a view with the negation still to be made: call its resolve_neg()", name);       // (the imaginary part of a conjugate)
     if (!t->is_cuda() || t->get_device() != e.index) refuse("%s must be on cuda:%d", name, e.index);
     if (type >= 0 && kind != type) refuse("%s is %s: must be %s", name, name_of(kind), name_of(type));
     const int64_t n = t->size(0), c = t->size(1), ld = n <= 1 ? c : t->stride(0);
@@ -82,6 +83,7 @@ void *vector(const Env &e, PyObject *o, const char *name, int64_t n, at::ScalarT
 {
     if (o == Py_None) return nullptr;
     const at::Tensor *t = THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+    if (t && t->is_neg()) refuse("%s is a view with the negation still to be made: call its resolve_neg()", name);
     if (!t || t->layout() != at::kStrided || t->dim() != 1 || t->size(0) != n || t->scalar_type() != s || !t->is_contiguous() || !t->is_cuda() || t->get_device() != e.index)
         refuse("%s must be a contiguous %s vector of %lld on cuda:%d", name, s == at::kFloat ? "torch.float32" : "torch.int32", (long long)n, e.index);
     return t->data_ptr();

@@ -51,3 +51,26 @@ def test_a_flag_without_a_truth_value_raises_its_own_error(eng):
                  lambda f: eng.linear_grad_weight(x, x, want_bias=f), lambda f: eng.softmax_loss(x, labels, want_grad=f)):
         with pytest.raises(LookupError, match="neither"):
             call(Neither())
+
+
+def test_views_that_are_still_to_be_negated_are_refused():
+    """The imaginary part of a conjugate is such a view: what lies in memory has the other sign."""
+    from opal_amd._lib import bind
+    b = bind()
+    z = torch.complex(torch.randn(3, 4), torch.randn(3, 4)).conj()
+    x = z.imag[:, :1]
+    assert x.is_neg() and not x.resolve_neg().is_neg()
+    for call in (lambda: b.softmax_class(0, 0, x), lambda: b.layer_norm(0, 0, x, None, None, 1e-5, None, False), lambda: b.linear_grad_weight(0, 0, x, x, True)):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
+
+
+@pytest.mark.gpu
+def test_vectors_that_are_still_to_be_negated_are_refused(eng):
+    z = torch.complex(torch.randn(1), torch.randn(1)).cuda().conj()
+    gamma = z.imag                             # one column: contiguous
+    x = torch.randn(5, 1, device="cuda")
+    with pytest.raises(ValueError, match="gamma.*resolve_neg"):
+        eng.layer_norm(x, gamma)
+    y, _, _ = eng.layer_norm(x, gamma.resolve_neg())
+    assert y.shape == (5, 1)
