@@ -4,6 +4,7 @@ torch is plumbing only (device memory, streams); every computation on the hot pa
 libopal_hip.so (hand-written HIP kernels for gfx950) through the C-ABI of include/opal_hip.h.
 """
 import ctypes as C
+import functools
 
 import numpy as np
 
@@ -211,7 +212,7 @@ class Engine:
         torch.cuda.set_device(self.device)
         stream = torch.cuda.current_stream(self.device).cuda_stream if use_torch_stream else None
         self._stream = stream or 0
-        self._lib, self._bind = lib(), bind()
+        self._lib = lib()
         # the handle of a device's current stream: the short way where torch has it (0.1 us against 1.9)
         self._current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
         self._index = self.device.index
@@ -220,6 +221,11 @@ class Engine:
         self._h, self._ctx = h, h.value
         self.k = self.P = self.t = 0
         self.K = self.bits = 0
+
+    @functools.cached_property
+    def _bind(self):
+        """The extension module of the score head's calls: loaded by the first of them, since nothing else needs it."""
+        return bind()
 
     def close(self):
         if getattr(self, "_h", None):

@@ -74,3 +74,25 @@ def test_vectors_that_are_still_to_be_negated_are_refused(eng):
         eng.layer_norm(x, gamma)
     y, _, _ = eng.layer_norm(x, gamma.resolve_neg())
     assert y.shape == (5, 1)
+
+
+def test_only_the_score_head_needs_its_extension_module(monkeypatch):
+    """An Engine comes up, and is used, where the extension is absent or does not load; the first call that needs it says so.  (No GPU: the
+    library and torch's streams are stand-ins.)"""
+    import types
+    import opal_amd.engine as engine
+
+    def absent():
+        raise ImportError("no extension here")
+    library = types.SimpleNamespace(opal_ctx_create=lambda *a: 0, opal_ctx_destroy=lambda h: 0, opal_sync=lambda h: 0)
+    monkeypatch.setattr(engine, "bind", absent)
+    monkeypatch.setattr(engine, "lib", lambda: library)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d: types.SimpleNamespace(cuda_stream=0))
+    e = engine.Engine(0)
+    e.sync()
+    for call in (lambda: e.softmax_class(None), lambda: e.linear(None, None), lambda: e.layer_norm(None)):
+        with pytest.raises(ImportError, match="no extension here"):
+            call()
+    e.close()
