@@ -1,10 +1,12 @@
 """ctypes binding of libopal_hip.so (include/opal_hip.h).  There is no fallback: if the library is missing or a
 call fails, this module raises."""
 import ctypes as C
+import hashlib
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libopal_hip.so")
+BIND_SOURCES = (os.path.join(_HERE, "csrc", "opal_bind.cpp"), os.path.join(os.path.dirname(_HERE), "include", "opal_hip.h"))
 
 OPAL_OK = 0
 OPAL_EINVAL = -22
@@ -94,14 +96,33 @@ def lib():
     return _lib
 
 
+def bind_source():
+    """Hash of what the extension module is made of, the C prototypes it is compiled against included; None where the sources are not there."""
+    h = hashlib.sha256()
+    try:
+        for path in BIND_SOURCES:
+            with open(path, "rb") as f:
+                h.update(os.path.basename(path).encode() + b"\0" + f.read() + b"\0")
+    except OSError:
+        return None
+    return h.hexdigest()[:16]
+
+
 def bind():
     """The extension module behind Engine's score head calls (csrc/opal_bind.cpp, built by __graft_entry__.build()); raises if it
-    is not there."""
+    is not there, or was built from other sources or for another torch than those at hand."""
     lib()                                      # first, and with torch, which the extension is linked to
+    import torch
+    build = "build it with `python -c 'import __graft_entry__ as g; g.build()'`"
     try:
         from . import _bind
     except ImportError as e:
-        raise ImportError("opal_amd/_bind.so (%s): build it with `python -c 'import __graft_entry__ as g; g.build()'`" % e) from e
+        raise ImportError("opal_amd/_bind.so (%s): %s" % (e, build)) from e
+    source = bind_source()
+    if source is not None and getattr(_bind, "source", None) != source:
+        raise ImportError("opal_amd/_bind.so is stale, built from other sources: " + build)
+    if _bind.torch != torch.__version__:
+        raise ImportError("opal_amd/_bind.so was built for torch %s, this is %s: %s" % (_bind.torch, torch.__version__, build))
     _bind.on_error(check)
     return _bind
 

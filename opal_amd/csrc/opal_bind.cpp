@@ -292,4 +292,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__bind() { return PyModule_Create(&module); }
+// What it was built from (a hash that the build computes) and for: opal_amd._lib.bind compares both.
+PyMODINIT_FUNC PyInit__bind()
+{
+    PyObject *m = PyModule_Create(&module);
+    if (m && (PyModule_AddStringConstant(m, "source", OPAL_BIND_SOURCE) || PyModule_AddStringConstant(m, "torch", OPAL_BIND_TORCH))) Py_CLEAR(m);
+    return m;
+}

@@ -96,3 +96,22 @@ def test_only_the_score_head_needs_its_extension_module(monkeypatch):
         with pytest.raises(ImportError, match="no extension here"):
             call()
     e.close()
+
+
+def test_a_stale_extension_module_is_noticed(monkeypatch):
+    """Built from other sources, or for another torch, than those at hand: refused, as a library that lacks a symbol is."""
+    from opal_amd import _lib
+    module = _lib.bind()
+    assert module.source == _lib.bind_source() and module.torch == torch.__version__
+    with monkeypatch.context() as m:
+        m.setattr(module, "torch", "1.0.0")
+        with pytest.raises(ImportError, match="for torch 1.0.0"):
+            _lib.bind()
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "bind_source", lambda: "another")
+        with pytest.raises(ImportError, match="stale"):
+            _lib.bind()
+    with monkeypatch.context() as m:                           # an installation without the sources
+        m.setattr(_lib, "BIND_SOURCES", ("/nowhere/opal_bind.cpp",))
+        assert _lib.bind_source() is None and _lib.bind() is module
+    assert _lib.bind() is module
