@@ -396,12 +396,14 @@ class Engine:
         # (an ExternalStream of handle 0 would be a new stream, not the default one)
         own = t.cuda.ExternalStream(self._stream, device=self.device) if self._stream else t.cuda.default_stream(self.device)
         own.wait_stream(cur)
-        # what the call allocates comes from the current stream's memory and goes back to it: later work there waits for the engine's
-        out = call(self._ctx, self._index, *tensors, *rest)
+        # results and workspaces come from the engine's own stream's memory: a workspace that goes back to it can only be handed out to work
+        # behind the call's (another thread may ask for memory on the current stream before that waits for the engine's)
+        with t.cuda.stream(own):
+            out = call(self._ctx, self._index, *tensors, *rest)
         cur.wait_stream(own)
-        for x in (*tensors, *out):             # their memory may be handed out again once the engine's stream is done with it
+        for x, user in [(x, own) for x in tensors] + [(x, cur) for x in out]:      # their memory may be handed out again once both streams are done with it
             if x is not None:
-                x.record_stream(own)
+                x.record_stream(user)
         return out
 
     def layer_norm(self, x, gamma=None, beta=None, eps=1e-5, out_dtype=None, want_stats=False):

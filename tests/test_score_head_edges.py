@@ -115,3 +115,51 @@ def test_a_stale_extension_module_is_noticed(monkeypatch):
         m.setattr(_lib, "BIND_SOURCES", ("/nowhere/opal_bind.cpp",))
         assert _lib.bind_source() is None and _lib.bind() is module
     assert _lib.bind() is module
+
+
+@pytest.mark.gpu
+def test_a_workspace_is_not_handed_out_while_the_engine_works(eng):
+    """With the engine on another stream than torch's current one: memory that a call gives back when it returns (its workspace) is not given to
+    the current stream, which waits for the engine's only after that."""
+    given = []
+
+    def call(ctx, index, x):
+        work = torch.empty(33 << 20, dtype=torch.uint8, device="cuda")           # a block of its own
+        given.append(work.data_ptr())
+        out = x + 1
+        del work
+        with torch.cuda.stream(side):                                            # as another thread would, between the call and the wait
+            given.append(torch.empty(33 << 20, dtype=torch.uint8, device="cuda").data_ptr())
+        return (out,)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    with torch.cuda.stream(side):
+        x = torch.zeros(1000, device="cuda")
+        out, = eng._run(call, (x,))
+        assert given[0] != given[1]
+        assert torch.equal(out, torch.ones(1000, device="cuda"))
+    side.synchronize()
+
+
+@pytest.mark.gpu
+def test_results_on_another_stream_keep_their_memory_until_it_is_done(eng):
+    """Results that are used on the current stream and dropped: the engine's next calls must not write over them first."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(4096, 700, device="cuda", generator=g).to(BF16)
+    dy = torch.randn(4096, 512, device="cuda", generator=g).to(BF16)
+    want = eng.linear_grad_weight(dy, x)
+    torch.cuda.synchronize()
+    side, heavy = torch.cuda.Stream(), torch.randn(4096, 4096, device="cuda")
+    with torch.cuda.stream(side):
+        kept = []
+        for i in range(6):
+            dw, db = eng.linear_grad_weight(dy, x)
+            for _ in range(3):
+                heavy @ heavy                  # work ahead of the results' use
+            kept.append((dw * 1.0, db * 1.0))
+            del dw, db
+            eng.linear_grad_weight(-dy, x)     # asks for memory of the same size at once
+    side.synchronize()
+    for dw, db in kept:
+        assert torch.equal(dw, want[0]) and torch.equal(db, want[1])
