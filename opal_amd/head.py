@@ -105,7 +105,7 @@ class ScoreHead:
             c, p = self.predict(scores)
             cls.append(c[:n])
             prob.append(p[:n])
-        return t.cat(cls), t.cat(prob)
+        return (t.cat(cls), t.cat(prob)) if cls else (t.empty(0, dtype=t.int32, device=e.device), t.empty(0, dtype=t.float32, device=e.device))
 
     def save(self, path):
         with open(path, "wb") as f:

@@ -163,3 +163,21 @@ def test_results_on_another_stream_keep_their_memory_until_it_is_done(eng):
     side.synchronize()
     for dw, db in kept:
         assert torch.equal(dw, want[0]) and torch.equal(db, want[1])
+
+
+# ------------------------------------------------------------------------------ the head itself (opal_amd/head.py)
+class HostEngine:
+    """What ScoreHead needs of an engine to hold parameters: no GPU."""
+    torch = torch
+    device = torch.device("cpu")
+    K = 5
+
+
+def test_answers_of_no_fragments():
+    from opal_amd.engine import DeviceBatch
+    from opal_amd.head import ScoreHead, batch_scores
+    head = ScoreHead(HostEngine, 5, 3)
+    empty = DeviceBatch(torch.empty(0, dtype=torch.uint8), torch.zeros(1, dtype=torch.int64), torch.zeros(1, dtype=torch.int32), 0, 0)
+    cls, prob = head.answers(empty, True)
+    assert cls.shape == (0,) and cls.dtype == torch.int32 and prob.shape == (0,) and prob.dtype == F32
+    assert list(batch_scores(HostEngine, empty, True)) == []
