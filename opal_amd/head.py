@@ -6,7 +6,7 @@ for a sister species.  The head reads all K scores s of a fragment,
     z = layer norm(s),   logits = z + W2 gelu(W1 z + b1) + b2,   p = softmax(logits),
 
 and is trained by cross entropy on fragments the linear model has scored, with AdaGrad as the linear learner uses.  It starts as the
-linear model itself (W2 = 0).  The work is Engine.layer_norm, linear, linear_grad_input, linear_grad_weight, softmax_loss and
+linear model itself (W2 = 0): the answers are the linear model's, up to scores that 32 bits of z cannot tell apart.  The work is Engine.layer_norm, linear, linear_grad_input, linear_grad_weight, softmax_loss and
 softmax_class (hand-written HIP kernels); torch holds the parameters and makes the parameter update, a few passes over them.
 No counterpart in the reference, whose answer is the argmax of the scores (opal.py:449-469)."""
 import os
@@ -56,11 +56,14 @@ class ScoreHead:
             h.copy_(self.params[n])
 
     def forward(self, scores, for_training=False):
-        """logits float32 [n, K] (and what backward needs) of scores float32 [n, K]."""
+        """logits float32 [n, K] (and what backward needs) of scores float32 [n, K].  An answer hangs on which of two close scores is the
+        higher one: there the z that is added to the product stays in 32 bits.  A training step adds the bfloat16 z that the product
+        takes, a pass over the scores less: its gradients are rounded to bfloat16 anyway."""
         e, t, p = self.engine, self.engine.torch, self.params
         z, mean, rstd = e.layer_norm(scores, p["gamma"], p["beta"], eps=EPS, out_dtype=t.bfloat16, want_stats=for_training)
         h, pre = e.linear(z, self._half["w1"], p["b1"], activation="gelu", want_pre=for_training)
-        logits, _ = e.linear(h, self._half["w2"], p["b2"], residual=z, out_dtype=t.float32)
+        added = z if for_training else e.layer_norm(scores, p["gamma"], p["beta"], eps=EPS, out_dtype=t.float32)[0]
+        logits, _ = e.linear(h, self._half["w2"], p["b2"], residual=added, out_dtype=t.float32)
         return (logits, (scores, z, mean, rstd, h, pre)) if for_training else logits
 
     def gradients(self, scores, labels):

@@ -181,3 +181,26 @@ def test_answers_of_no_fragments():
     cls, prob = head.answers(empty, True)
     assert cls.shape == (0,) and cls.dtype == torch.int32 and prob.shape == (0,) and prob.dtype == F32
     assert list(batch_scores(HostEngine, empty, True)) == []
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,K", [(1, 5), (700, 63), (3000, 356), (16384, 1563)])
+def test_a_fresh_head_answers_as_the_linear_model(eng, n, K):
+    """Also where the two highest scores are close: 2^-16 apart, which 16 bits cannot tell.  In 32 bits a score of less than 4, less its mean and
+    scaled, is off by at most 4 (2^-24 + 2 2^-24) of the scale, twice that between two of them: 2^-18.4."""
+    from opal_amd.head import ScoreHead
+    g = torch.Generator().manual_seed(n + K)
+    s = (torch.randn(n, K, generator=g) * 0.3 - 0.6).clamp(-1, 1)
+    pair = torch.rand(n, K, generator=g).argsort(1)[:, :2]                       # two classes, the first of them a little above the other
+    top = 1 + torch.rand(n, generator=g)
+    s.scatter_(1, pair, torch.stack([top, top - 2.0 ** -16], 1))
+    head = ScoreHead(eng, K, 16, seed=1)
+    cls, prob = head.predict(s.cuda())
+    assert torch.equal(cls.cpu().long() - 1, pair[:, 0])
+    # the difference of two z is off by 24 U rstd (above) and by rstd's own error, (K + 8) U of it; the sum of K exponentials by (K + 8) U
+    U, d = 2.0 ** -24, s.double()
+    rstd = (d.var(1, unbiased=False, keepdim=True) + 1e-5).rsqrt()
+    z = (d - d.mean(1, keepdim=True)) * rstd
+    p = torch.softmax(z, 1).amax(1)
+    tol = ((K + 8) * (1 + z.amax(1) - z.amin(1)) + 24 * rstd[:, 0]) * U
+    assert ((prob.cpu().double() - p).abs() <= tol * p).all()
