@@ -9,18 +9,31 @@ and is trained by cross entropy on fragments the linear model has scored, with A
 linear model itself (W2 = 0): the answers are the linear model's, up to scores that 32 bits of z cannot tell apart.  The work is Engine.layer_norm, linear, linear_grad_input, linear_grad_weight, softmax_loss and
 softmax_class (hand-written HIP kernels); torch holds the parameters and makes the parameter update, a few passes over them.
 No counterpart in the reference, whose answer is the argmax of the scores (opal.py:449-469)."""
+import hashlib
 import os
 import struct
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 
-__all__ = ["ScoreHead", "HEAD_FILE", "batch_scores"]
+__all__ = ["ScoreHead", "HEAD_FILE", "batch_scores", "model_digest"]
 
 HEAD_FILE = "vw-model_final.head"        # next to vw-model_final.model
-_HDR = struct.Struct("<8sIII")           # magic, version, K, hidden; then float32 gamma, beta, w1, b1, w2, b2
+_HDR = struct.Struct("<8sIII")           # magic, version, K, hidden; version 2: model_digest; then float32 gamma, beta, w1, b1, w2, b2
+_DIGEST = 32                             # bytes
 _MAGIC = b"OPALHEAD"
 _NAMES = ("gamma", "beta", "w1", "b1", "w2", "b2")
 EPS = 1e-5
+
+
+def model_digest(path, piece=1 << 26):
+    """What tells a linear model's file from another: sha256 of the sha256 of its pieces (of 64 MiB, side by side)."""
+    def part(at):
+        with open(path, "rb") as f:
+            f.seek(at)
+            return hashlib.sha256(f.read(piece)).digest()
+    with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        return hashlib.sha256(b"".join(pool.map(part, range(0, os.path.getsize(path), piece)))).digest()
 
 
 def batch_scores(engine, batch, reverse, limit=1 << 30):
@@ -110,28 +123,48 @@ class ScoreHead:
             prob.append(p[:n])
         return (t.cat(cls), t.cat(prob)) if cls else (t.empty(0, dtype=t.int32, device=e.device), t.empty(0, dtype=t.float32, device=e.device))
 
-    def save(self, path):
+    def save(self, path, model=None):
+        """model: the file of the linear model that the head was trained behind; load() then knows it from another."""
         with open(path, "wb") as f:
-            f.write(_HDR.pack(_MAGIC, 1, self.K, self.hidden))
+            f.write(_HDR.pack(_MAGIC, 1 if model is None else 2, self.K, self.hidden))
+            if model is not None:
+                f.write(model_digest(model))
             for n in _NAMES:
                 self.params[n].cpu().numpy().tofile(f)
+
+    @staticmethod
+    def _header(f, path):
+        """(K, hidden, the model's digest or None) from the beginning of a head file; RuntimeError for anything else."""
+        raw = f.read(_HDR.size)
+        if len(raw) < _HDR.size or raw[:8] != _MAGIC:
+            raise RuntimeError("%s is not an opal_amd score head" % path)
+        _, version, K, hidden = _HDR.unpack(raw)
+        if version not in (1, 2) or not 1 <= K <= 1 << 20 or not 1 <= hidden <= 1 << 20:
+            raise RuntimeError("unsupported opal_amd score head in %s" % path)
+        if os.fstat(f.fileno()).st_size != _HDR.size + (version == 2) * _DIGEST + 4 * sum(int(np.prod(s)) for s in ScoreHead._shapes(K, hidden).values()):
+            raise RuntimeError("truncated head file " + path)
+        return K, hidden, f.read(_DIGEST) if version == 2 else None
+
+    @staticmethod
+    def _shapes(K, hidden):
+        return dict(gamma=(K,), beta=(K,), w1=(hidden, K), b1=(hidden,), w2=(K, hidden), b2=(K,))
 
     @staticmethod
     def read(path):
         """(K, hidden, parameters) of a head file; RuntimeError for anything else."""
         with open(path, "rb") as f:
-            raw = f.read(_HDR.size)
-            if len(raw) < _HDR.size or raw[:8] != _MAGIC:
-                raise RuntimeError("%s is not an opal_amd score head" % path)
-            _, version, K, hidden = _HDR.unpack(raw)
-            if version != 1 or not 1 <= K <= 1 << 20 or not 1 <= hidden <= 1 << 20:
-                raise RuntimeError("unsupported opal_amd score head in %s" % path)
-            shapes = dict(gamma=(K,), beta=(K,), w1=(hidden, K), b1=(hidden,), w2=(K, hidden), b2=(K,))
-            if os.fstat(f.fileno()).st_size != _HDR.size + 4 * sum(int(np.prod(s)) for s in shapes.values()):
-                raise RuntimeError("truncated head file " + path)
+            K, hidden, _ = ScoreHead._header(f, path)
+            shapes = ScoreHead._shapes(K, hidden)
             return K, hidden, {n: np.fromfile(f, dtype=np.float32, count=int(np.prod(shapes[n]))).reshape(shapes[n]) for n in _NAMES}
 
     @staticmethod
-    def load(engine, path):
+    def load(engine, path, model=None):
+        """model: the file of the linear model that is to be used; RuntimeError when the head was trained behind another (a head that was
+        saved without one is taken as it is)."""
+        if model is not None:
+            with open(path, "rb") as f:
+                trained_behind = ScoreHead._header(f, path)[2]
+            if trained_behind is not None and trained_behind != model_digest(model):
+                raise RuntimeError("%s was trained behind another model than %s: train it anew (train --head) or answer without it (predict --no-head)" % (path, model))
         K, hidden, params = ScoreHead.read(path)
         return ScoreHead(engine, K, hidden, params=params)

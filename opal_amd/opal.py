@@ -401,7 +401,7 @@ def train(ref_dir, model_dir, args, engine=None):
         if multipass:
             eng.load_weights(w, num_labels, bits)            # the saved regressor, which need not be the last pass's
         head = train_head(eng, genomes, genome_len, genome_taxid, dico, num_labels, args, log)
-        head.save(head_file)
+        head.save(head_file, model=final_model_file)
     log.write("saved %s (%d non-zero weights)\n" % (final_model_file, nnz))
     log.close()
     print("------------------------------------------------\nTotal wall clock runtime (sec): {}\n"
@@ -597,7 +597,7 @@ def predict(model_dir, test_dir, predict_dir, args, engine=None, chunk_bytes=Non
     head = None
     head_file = os.path.join(model_dir, HEAD_FILE)
     if os.path.exists(head_file) and not getattr(args, "no_head", False):
-        head = ScoreHead.load(eng, head_file)
+        head = ScoreHead.load(eng, head_file, model=model)
         if head.K != hdr["K"]:
             raise RuntimeError("%s has %d classes, the model %d" % (head_file, head.K, hdr["K"]))
     want_prob = bool(getattr(args, "probabilities", False))

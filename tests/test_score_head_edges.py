@@ -204,3 +204,62 @@ def test_a_fresh_head_answers_as_the_linear_model(eng, n, K):
     p = torch.softmax(z, 1).amax(1)
     tol = ((K + 8) * (1 + z.amax(1) - z.amin(1)) + 24 * rstd[:, 0]) * U
     assert ((prob.cpu().double() - p).abs() <= tol * p).all()
+
+
+def test_a_head_knows_its_model(tmp_path):
+    """A model of the same classes that was put in the place of the one the head was trained behind is noticed."""
+    from opal_amd.head import ScoreHead, model_digest
+    model, head_file = tmp_path / "m.model", str(tmp_path / "m.head")
+    model.write_bytes(bytes(range(256)) * 40)
+    ScoreHead(HostEngine, 5, 3, seed=2).save(head_file, model=str(model))
+    assert ScoreHead.load(HostEngine, head_file, model=str(model)).K == 5 and ScoreHead.load(HostEngine, head_file).hidden == 3
+    whole = model.read_bytes()
+    assert model_digest(str(model), piece=100) != model_digest(str(model), piece=1 << 20)      # pieces count, and are 64 MiB
+    for at in (0, 5000, len(whole) - 1):
+        model.write_bytes(whole[:at] + bytes([whole[at] ^ 1]) + whole[at + 1:])
+        with pytest.raises(RuntimeError, match="another model"):
+            ScoreHead.load(HostEngine, head_file, model=str(model))
+    for other in (whole[:-1], whole + b"x", b""):
+        model.write_bytes(other)
+        with pytest.raises(RuntimeError, match="another model"):
+            ScoreHead.load(HostEngine, head_file, model=str(model))
+    model.write_bytes(whole)
+    assert torch.equal(ScoreHead.load(HostEngine, head_file, model=str(model)).params["w1"], ScoreHead(HostEngine, 5, 3, seed=2).params["w1"])
+    raw = open(head_file, "rb").read()
+    for bad in (raw[:-1], raw + b"x", raw[:8] + b"\x03" + raw[9:], raw[:8] + b"\x01" + raw[9:], raw[:30]):
+        open(head_file, "wb").write(bad)
+        with pytest.raises(RuntimeError):
+            ScoreHead.load(HostEngine, head_file, model=str(model))
+        with pytest.raises(RuntimeError):
+            ScoreHead.read(head_file)
+    ScoreHead(HostEngine, 5, 3).save(head_file)                                    # without a model: as it is
+    assert ScoreHead.load(HostEngine, head_file, model=str(model)).K == 5
+
+
+@pytest.mark.gpu
+def test_predict_refuses_the_head_of_another_model(tmp_path):
+    import argparse
+    import numpy as np
+    from opal_amd import model as model_io, opal
+    from opal_amd.head import HEAD_FILE, ScoreHead
+    rng = np.random.default_rng(3)
+    K, bits = 5, 16
+    for d in ("model", "test"):
+        os.makedirs(tmp_path / d)
+    with open(os.path.join(os.path.dirname(os.path.abspath(__file__)), "golden", "patterns_k64_t16_m1_s7.txt")) as f:
+        (tmp_path / "model" / "patterns.txt").write_text(f.read())
+    (tmp_path / "model" / "vw-dico.txt").write_text("".join("tax%d\t%d\n" % (i, i) for i in range(1, K + 1)))
+    (tmp_path / "test" / "reads.fasta").write_text("".join(">r%d\n%s\n" % (i, "".join(rng.choice(list("ACGT"), size=120))) for i in range(20)))
+    model = str(tmp_path / "model" / "vw-model_final.model")
+    weights = [(rng.standard_normal(1 << bits) * 0.05).astype(np.float32) for _ in range(2)]
+    model_io.save_model(model, weights[0], K, bits)
+    ScoreHead(HostEngine, K, 4, seed=1).save(str(tmp_path / "model" / HEAD_FILE), model=model)
+
+    def predict(out, **more):
+        opal.predict(str(tmp_path / "model"), str(tmp_path / "test"), str(tmp_path / out), argparse.Namespace(kmer=64, reverse_complement=True, **more))
+        return (tmp_path / out / "test.fragments-db.preds.taxid").read_text().split()
+    assert predict("a") == predict("b", no_head=True)                              # a fresh head: the linear model's answers
+    model_io.save_model(model, weights[1], K, bits)
+    with pytest.raises(RuntimeError, match="another model"):
+        predict("c")
+    assert len(predict("d", no_head=True)) == 20
