@@ -137,8 +137,8 @@ def test_linear_gradients(eng, t, n, k, m, pad):
     assert none is None and torch.equal(dw, dw2)
 
 
-# enough rows and columns for the 256 x 256 tiles of 16-bit products: sums that end inside a step, a chunk, a stage of 64; columns that
-# end inside a group of eight; several tiles a block; every epilogue
+# enough rows and columns for the larger tiles of 16-bit products: sums that end inside a step, a chunk, a stage of 64; columns that
+# end inside a group of eight; several tiles a block (every epilogue of every kernel: test_score_head_kernels.py)
 BIG_SHAPES = [(16700, 100, 520), (33000, 71, 250), (11000, 40, 1563), (16500, 1, 512), (8200, 355, 1030), (70001, 33, 257), (16400, 192, 511), (9000, 1563, 1040), (33000, 1027, 500), (131000, 259, 300)]
 
 
