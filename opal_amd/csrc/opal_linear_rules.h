@@ -62,7 +62,10 @@ inline int product_tile(int product, int type, uint64_t M, uint64_t N, uint64_t 
 
 // Splits of the sum over the rows, none empty.  256 x 256 tiles: as many as give the 256 CUs a tile each, of at least 16 steps.
 // Smaller ones: two blocks per CU, of at least four steps; 128 x 128 from twelve on: 20 000 x 512 x 512 (16 tiles) 16.3 us against 22.3 with 64 x
-// 64, 6000 x 1564 x 512 (52) 16.8 against 22.0; below it 8192 x 512 x 256 (8) 9.2 against 7.1, 20 000 x 355 x 128 (3) 12.1 against 7.5.  Few rows, while 32 x 32 tiles find a CU each, are one block's for all of the
+// 64, 6000 x 1564 x 512 (52) 16.8 against 22.0; below it 8192 x 512 x 256 (8) 9.2 against 7.1, 20 000 x 355 x 128 (3) 12.1 against 7.5.  32-bit types from 6000
+// steps of all tiles together on, and not where they reach a quarter further: 100 000 x 1564 x 512 (162 500) 1389 against 1706, 6000 x 1564 x 512 (9776)
+// 98 against 109, 4096 x 1564 x 512 (6656) 75 against 77, 16 384 x 356 x 512 (6144) 65 against 64 (rows not on 16 bytes: 95 against 122); below it 6000 x
+// 356 x 512 (2256) 35 against 30, 3000 x 520 x 400 (1880) 36 against 23; 50 000 x 130 x 1564, a third further, 335 against 292.  Few rows, while 32 x 32 tiles find a CU each, are one block's for all of the
 // sum, without splits to add up: 1999 x 355 x 63 (rows, in, out) 5.3 us against 4.8 and 4.6 for the splits' sum; 4096 x 355 x 128 8.8 against
 // 10.2 + 4.6, 8192 x 355 x 128 26 against 10.6 + 4.6; 32-bit types, whose operands are loads of one column, 1024 x 512 x 512 10.0 against 13.6 +
 // 4.6, 1024 x 384 x 64 9.8 against 5.5 + 4.6, 1999 x 355 x 63 15.7 against 5.9 + 4.6.  The choice does not look at the operands' alignment, so that the workspace
@@ -76,7 +79,9 @@ inline Splits weight_splits(uint64_t n, uint32_t in, uint32_t out, int type)
     const uint64_t steps = std::max<uint64_t>((n + step - 1) / step, 1);
     const uint64_t big = tiles_of(out, in, 2);
     const bool large = n > 0 && type != OPAL_F32 && in > 128 && out > 128 && steps * big >= 16 * 128;
-    const int tile = large ? 2 : in > 64 && out > 64 && tiles_of(out, in, 1) >= 12 ? 1 : 0;
+    const uint64_t t128 = tiles_of(out, in, 1);
+    const bool middle = type == OPAL_F32 ? steps * t128 >= 6000 && t128 * 16 <= tiles_of(out, in, 0) * 5 : in > 64 && out > 64 && t128 >= 12;
+    const int tile = large ? 2 : middle ? 1 : 0;
     uint64_t s = large ? std::min<uint64_t>(256 / std::min<uint64_t>(big, 256), steps / 16) : std::min<uint64_t>(512 / std::min<uint64_t>(tiles_of(out, in, tile), 512), steps / 4);
     s = std::max<uint64_t>(s, 1);
     const uint64_t per = (steps + s - 1) / s;

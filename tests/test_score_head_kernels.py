@@ -99,6 +99,12 @@ def test_the_sizes_below_reach_the_kernels_they_are_for(rules):
         assert rules(["weight %d %d %d 0" % (n, k, m)])[0][0] == MIDDLE
 
 
+def test_weight_gradients_in_32_bits_take_128_tiles_where_those_were_faster(rules):
+    for n, k, m, tile in ((100000, 1564, 512, MIDDLE), (6000, 1564, 512, MIDDLE), (4096, 1564, 512, MIDDLE), (16384, 356, 512, MIDDLE), (100000, 200, 1000, MIDDLE),
+                          (6000, 356, 512, SMALL), (3000, 520, 400, SMALL), (4096, 356, 512, SMALL), (50000, 130, 1564, SMALL), (100000, 63, 64, SMALL)):
+        assert rules(["weight %d %d %d 0" % (n, k, m)])[0][0] == tile, (n, k, m)
+
+
 def random(g, t):
     """rnd(rows, cols, scale, rows on 16 bytes): a matrix whose gaps are NaN"""
     def rnd(a, b, scale=1.0, aligned=True, t=t):
