@@ -3,6 +3,7 @@
 torch is plumbing only (device memory, streams); every computation on the hot path happens inside
 libopal_hip.so (hand-written HIP kernels for gfx950) through the C-ABI of include/opal_hip.h.
 """
+import contextlib
 import ctypes as C
 import functools
 
@@ -389,22 +390,34 @@ class Engine:
         """One call on the engine's stream, ordered with torch's current stream when that is another one."""
         if self._current(self._index) == self._stream:
             return call(self._ctx, self._index, *tensors, *rest)
-        t = self.torch
+        # results and workspaces come from the engine's own stream's memory: a workspace that goes back to it can only be handed out to work
+        # behind the call's (another thread may ask for memory on the current stream before that waits for the engine's)
+        with self._own_stream(inputs=tensors) as results:
+            out = call(self._ctx, self._index, *tensors, *rest)
+            results += out
+        return out
+
+    @contextlib.contextmanager
+    def _own_stream(self, inputs=()):
+        """What stands inside runs on the engine's stream: behind the work of torch's current stream where that is another one, and ahead of what
+        comes there afterwards.  inputs: the current stream's tensors that are used inside (None among them is fine); what is
+        appended to the list that this yields is used outside."""
+        t, results = self.torch, []
+        if self._current(self._index) == self._stream:
+            yield results
+            return
         cur = t.cuda.current_stream(self.device)
         if t.cuda.is_current_stream_capturing():
             raise RuntimeError("capture on the stream the Engine was created under: its calls run there")
         # (an ExternalStream of handle 0 would be a new stream, not the default one)
         own = t.cuda.ExternalStream(self._stream, device=self.device) if self._stream else t.cuda.default_stream(self.device)
         own.wait_stream(cur)
-        # results and workspaces come from the engine's own stream's memory: a workspace that goes back to it can only be handed out to work
-        # behind the call's (another thread may ask for memory on the current stream before that waits for the engine's)
         with t.cuda.stream(own):
-            out = call(self._ctx, self._index, *tensors, *rest)
+            yield results
         cur.wait_stream(own)
-        for x, user in [(x, own) for x in tensors] + [(x, cur) for x in out]:      # their memory may be handed out again once both streams are done with it
+        for x, user in [(x, own) for x in inputs] + [(x, cur) for x in results]:   # their memory may be handed out again once both streams are done with it
             if x is not None:
                 x.record_stream(user)
-        return out
 
     def layer_norm(self, x, gamma=None, beta=None, eps=1e-5, out_dtype=None, want_stats=False):
         """y = (x - mean) rstd gamma + beta per row (opal_layer_norm).  Returns (y, mean, rstd); mean and rstd are None unless

@@ -43,7 +43,10 @@ def batch_scores(engine, batch, reverse, limit=1 << 30):
     for lo in range(0, batch.n, rows):
         hi = min(batch.n, lo + rows)
         part = DeviceBatch(batch.data, batch.off[lo:hi], batch.len[lo:hi], hi - lo, batch.nbytes)
-        yield lo, engine.predict(part, reverse, want_scores=True)[1]
+        with engine._own_stream(inputs=(part.data, part.off, part.len)) as results:
+            scores = engine.predict(part, reverse, want_scores=True)[1]
+            results.append(scores)
+        yield lo, scores
 
 
 class ScoreHead:
@@ -111,17 +114,21 @@ class ScoreHead:
         how many others its piece of the file holds."""
         from .engine import DeviceBatch
         e, t = self.engine, self.engine.torch
+        if batch.n == 0:
+            return t.empty(0, dtype=t.int32, device=e.device), t.empty(0, dtype=t.float32, device=e.device)
         rows = max(1, min(rows, limit // (4 * self.K)))
         cls, prob = [], []
-        scores = t.empty((rows, self.K), dtype=t.float32, device=e.device)
-        for lo in range(0, batch.n, rows):
-            n = min(batch.n - lo, rows)
-            e.predict(DeviceBatch(batch.data, batch.off[lo:lo + n], batch.len[lo:lo + n], n, batch.nbytes), reverse, want_scores=True, out_scores=scores)
-            scores[n:].zero_()
-            c, p = self.predict(scores)
-            cls.append(c[:n])
-            prob.append(p[:n])
-        return (t.cat(cls), t.cat(prob)) if cls else (t.empty(0, dtype=t.int32, device=e.device), t.empty(0, dtype=t.float32, device=e.device))
+        with e._own_stream(inputs=(batch.data, batch.off, batch.len)) as results:
+            scores = t.empty((rows, self.K), dtype=t.float32, device=e.device)
+            for lo in range(0, batch.n, rows):
+                n = min(batch.n - lo, rows)
+                e.predict(DeviceBatch(batch.data, batch.off[lo:lo + n], batch.len[lo:lo + n], n, batch.nbytes), reverse, want_scores=True, out_scores=scores)
+                scores[n:].zero_()
+                c, p = self.predict(scores)
+                cls.append(c[:n])
+                prob.append(p[:n])
+            results += [t.cat(cls), t.cat(prob)]
+        return tuple(results)
 
     def save(self, path, model=None):
         """model: the file of the linear model that the head was trained behind; load() then knows it from another."""

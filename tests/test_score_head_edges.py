@@ -263,3 +263,40 @@ def test_predict_refuses_the_head_of_another_model(tmp_path):
     with pytest.raises(RuntimeError, match="another model"):
         predict("c")
     assert len(predict("d", no_head=True)) == 20
+
+
+@pytest.mark.gpu
+def test_answers_on_another_stream_wait_for_the_fragments(eng):
+    """Fragments that the current stream is still bringing when it asks for their scores or answers; the engine runs on another one."""
+    import numpy as np
+    import opal_amd
+    from opal_amd.engine import DeviceBatch
+    from opal_amd.head import ScoreHead, batch_scores
+    rng = np.random.default_rng(11)
+    K, bits, n = 24, 16, 500
+    e = opal_amd.Engine(0)
+    e.set_patterns(np.array([range(8), range(0, 16, 2)], dtype=np.int32), 16)
+    e.load_weights((rng.standard_normal(1 << bits) * 0.1).astype(np.float32), K, bits)
+    e.set_vw_options()
+    text = "".join(">r%d\n%s\n" % (i, "".join(rng.choice(list("ACGT"), size=100))) for i in range(n))
+    batch = e.ingest_fasta(np.frombuffer(text.encode(), dtype=np.uint8).copy())
+    head = ScoreHead(e, K, 16, seed=5)
+    want = head.answers(batch, True, rows=512)
+    scores = torch.cat([s for _, s in batch_scores(e, batch, True, limit=4 * K * 200)])
+    none = head.answers(DeviceBatch(torch.zeros_like(batch.data), batch.off, batch.len, n, batch.nbytes), True, rows=512)
+    assert not torch.equal(none[0], want[0])
+    torch.cuda.synchronize()
+    side, heavy = torch.cuda.Stream(), torch.randn(8192, 8192, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for ask in (lambda b: head.answers(b, True, rows=512), lambda b: (torch.cat([s for _, s in batch_scores(e, b, True, limit=4 * K * 200)]),)):
+            late = DeviceBatch(torch.zeros_like(batch.data), batch.off, batch.len, n, batch.nbytes)
+            for _ in range(10):
+                heavy @ heavy
+            late.data.copy_(batch.data)
+            got = [x.clone() for x in ask(late)]
+            late.data.zero_()                  # behind the answers
+            side.synchronize()
+            for a, b in zip(got, want if len(got) == 2 else (scores,)):
+                assert torch.equal(a, b)
+    e.close()
