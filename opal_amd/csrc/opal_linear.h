@@ -55,7 +55,7 @@ __device__ __forceinline__ float act_value(float v, int act)
 
 __device__ __forceinline__ float act_slope(float v, int act)
 {
-    if (act == ACT_RELU) return v > 0.f ? 1.f : 0.f;
+    if (act == ACT_RELU) return v > 0.f ? 1.f : 0.f;      // NaN, whose result is NaN, passes nothing on
     const float c = fminf(fmaxf(v, -64.f), 64.f);      // beyond it p is 0 or 1 and c^2 p (1 - p) must not become 0 inf
     if (act == ACT_SILU) {
         const float p = sigmoid(v);

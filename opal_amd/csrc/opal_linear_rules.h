@@ -66,7 +66,8 @@ inline int product_tile(int product, int type, uint64_t M, uint64_t N, uint64_t 
 // steps of all tiles together on, and not where they reach a quarter further: 100 000 x 1564 x 512 (162 500) 1389 against 1706, 6000 x 1564 x 512 (9776)
 // 98 against 109, 4096 x 1564 x 512 (6656) 75 against 77, 16 384 x 356 x 512 (6144) 65 against 64 (rows not on 16 bytes: 95 against 122); below it 6000 x
 // 356 x 512 (2256) 35 against 30, 3000 x 520 x 400 (1880) 36 against 23; 50 000 x 130 x 1564, a third further, 335 against 292.  Few rows, while 32 x 32 tiles find a CU each, are one block's for all of the
-// sum, without splits to add up: 1999 x 355 x 63 (rows, in, out) 5.3 us against 4.8 and 4.6 for the splits' sum; 4096 x 355 x 128 8.8 against
+// sum, without splits to add up: 1999 x 355 x 63 (rows, in, out) 6.0 us a call with operands in the caches (8.7 from memory)
+// against 4.8 and 4.6 for the splits' sum; 4096 x 355 x 128 8.8 against
 // 10.2 + 4.6, 8192 x 355 x 128 26 against 10.6 + 4.6; 32-bit types, whose operands are loads of one column, 1024 x 512 x 512 10.0 against 13.6 +
 // 4.6, 1024 x 384 x 64 9.8 against 5.5 + 4.6, 1999 x 355 x 63 15.7 against 5.9 + 4.6.  The choice does not look at the operands' alignment, so that the workspace
 // does not depend on it; unaligned operands take 128 x 128 tiles in the same splits.  256 x 256 tiles ask for chunks ahead of the first step and need one: a

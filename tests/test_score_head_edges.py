@@ -165,6 +165,23 @@ def test_results_on_another_stream_keep_their_memory_until_it_is_done(eng):
         assert torch.equal(dw, want[0]) and torch.equal(db, want[1])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("n", [3, 300])
+def test_relu_and_nan(eng, t, n):
+    """As the header says: NaN stays NaN, and neither it nor 0 passes a gradient on."""
+    nan = float("nan")
+    x = torch.randn(n, 24, device="cuda").to(t)
+    w = torch.eye(24, device="cuda").to(t)
+    x[1, 5], x[2] = nan, 0.0
+    y, pre = eng.linear(x, w, activation="relu", want_pre=True)
+    assert y[1].isnan().all() and not y[2].any() and torch.equal(y[0], x[0].clamp(min=0))         # (NaN times 0 is in each of the row's sums)
+    pre = pre.clone()
+    pre[1] = nan
+    dx = eng.linear_grad_input(torch.ones(n, 24, device="cuda").to(t), w, pre=pre, activation="relu")
+    assert not dx[1].any() and not dx[2].any() and torch.equal(dx[0], (x[0] > 0).to(t))
+
+
 # ------------------------------------------------------------------------------ the head itself (opal_amd/head.py)
 class HostEngine:
     """What ScoreHead needs of an engine to hold parameters: no GPU."""
