@@ -1,13 +1,14 @@
 """The score head: a trained layer behind the linear model's per-class scores (`train --head H`, `predict`).
 
 The linear model is K independent regressors: its scores are no probabilities and nothing corrects a class that is regularly taken
-for a sister species.  The head reads all K scores s of a fragment,
+for a sister species.  (On reads of strains that neither has seen the head has not made the answers better, 0.9954 against 0.9972 of 64 species: what it
+gives is a probability that orders them.)  The head reads all K scores s of a fragment,
 
     z = layer norm(s),   logits = z + W2 gelu(W1 z + b1) + b2,   p = softmax(logits),
 
 and is trained by cross entropy on fragments the linear model has scored, with AdaGrad as the linear learner uses.  It starts as the
-linear model itself (W2 = 0): the answers are the linear model's, up to scores that 32 bits of z cannot tell apart.  The work is Engine.layer_norm, linear, linear_grad_input, linear_grad_weight, softmax_loss and
-softmax_class (hand-written HIP kernels); torch holds the parameters and makes the parameter update, a few passes over them.
+linear model itself (W2 = 0): the answers are the linear model's, up to scores that 32 bits of z cannot tell apart.  The work is
+Engine.layer_norm, linear, linear_grad_input, linear_grad_weight, softmax_loss and softmax_class (hand-written HIP kernels); torch holds the parameters and makes the parameter update, a few passes over them.
 No counterpart in the reference, whose answer is the argmax of the scores (opal.py:449-469)."""
 import hashlib
 import os
