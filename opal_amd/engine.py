@@ -401,7 +401,7 @@ class Engine:
     @contextlib.contextmanager
     def _own_stream(self, inputs=()):
         """What stands inside runs on the engine's stream: behind the work of torch's current stream where that is another one, and ahead of what
-        comes there afterwards.  inputs: the current stream's tensors that are used inside (None among them is fine); what is
+        comes there afterwards.  inputs: the current stream's tensors that are used inside (what is no tensor on the GPU is passed over); what is
         appended to the list that this yields is used outside."""
         t, results = self.torch, []
         if self._current(self._index) == self._stream:
@@ -413,12 +413,14 @@ class Engine:
         # (an ExternalStream of handle 0 would be a new stream, not the default one)
         own = t.cuda.ExternalStream(self._stream, device=self.device) if self._stream else t.cuda.default_stream(self.device)
         own.wait_stream(cur)
-        with t.cuda.stream(own):
-            yield results
-        cur.wait_stream(own)
-        for x, user in [(x, own) for x in inputs] + [(x, cur) for x in results]:   # their memory may be handed out again once both streams are done with it
-            if x is not None:
-                x.record_stream(user)
+        try:
+            with t.cuda.stream(own):
+                yield results
+        finally:                               # what was launched before an error runs all the same
+            cur.wait_stream(own)
+            for x, user in [(x, own) for x in inputs] + [(x, cur) for x in results]:   # their memory may be handed out again once both streams are done with it
+                if isinstance(x, t.Tensor) and x.is_cuda:
+                    x.record_stream(user)
 
     def layer_norm(self, x, gamma=None, beta=None, eps=1e-5, out_dtype=None, want_stats=False):
         """y = (x - mean) rstd gamma + beta per row (opal_layer_norm).  Returns (y, mean, rstd); mean and rstd are None unless

@@ -143,6 +143,19 @@ def test_a_workspace_is_not_handed_out_while_the_engine_works(eng):
 
 
 @pytest.mark.gpu
+def test_refusals_on_another_stream_are_the_refusals(eng):
+    """An argument that is no tensor, or is on the CPU, is refused as it is on the engine's stream; the streams stay in order."""
+    x, w = torch.randn(4, 8, device="cuda"), torch.randn(6, 8, device="cuda")
+    want = eng.linear(x, w)[0]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()) as _:
+        for call in (lambda: eng.linear(x, [1.0]), lambda: eng.linear(x.cpu(), w), lambda: eng.linear(x, None), lambda: eng.softmax_class(None)):
+            with pytest.raises(ValueError):
+                call()
+        assert torch.equal(eng.linear(x, w)[0], want)
+
+
+@pytest.mark.gpu
 def test_results_on_another_stream_keep_their_memory_until_it_is_done(eng):
     """Results that are used on the current stream and dropped: the engine's next calls must not write over them first."""
     g = torch.Generator(device="cuda").manual_seed(7)
